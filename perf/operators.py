@@ -179,7 +179,7 @@ def _act(z, act):
     if act == "none":
         return z
     if act == "relu":
-        return torch.where(z > 0, z, torch.zeros_like(z))
+        return torch.where(z < 0, torch.zeros_like(z), z)
     if act == "silu":
         return z / (1.0 + torch.exp(-z))
     if act == "gelu":
@@ -191,7 +191,7 @@ def _act_grad(z, act):
     if act == "none":
         return torch.ones_like(z)
     if act == "relu":
-        return (z > 0).to(z.dtype)
+        return 1.0 - (z <= 0).to(z.dtype)
     if act == "silu":
         sig = 1.0 / (1.0 + torch.exp(-z))
         return sig * (1.0 + z * (1.0 - sig))
