@@ -1,0 +1,538 @@
+// linear.cu - the entry points of the feed-forward operators (cudair_linear,
+// cudair_gated and their gradients): argument rules, the products they are made of,
+// and the element-wise step of the gradients.
+//
+// The gradients' element-wise step (act_grad_kernel):
+//   linear  dZ = dY * act'(Z),  dbias[n] = sum_m dZ[m, n]
+//   gated   dG = dH * U * act'(G),  dU = dH * act(G)
+// dZ, dG and dU are then operands of two tensor-core products each, so they
+// are rounded to 16 bits once here: doing it inside the products would repeat the
+// activation for every tile that reads them.  Bound by HBM: 6 bytes an element
+// (linear: two reads, one write), 10 (gated: three reads, two writes).
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include "cudair_internal.h"
+#include "linear_epilogue.cuh"
+#include "linear_internal.h"
+#include "sm100.cuh"
+
+namespace cudair {
+namespace ffn {
+
+constexpr int EW_THREADS = 256;
+constexpr int EW_COLS = 64;              // columns per block: 8 threads of 8 columns
+constexpr int EW_ROWS = EW_THREADS / 8;  // rows per step of a block
+constexpr int EW_BATCH = 4;              // steps whose loads are issued together
+
+struct EwArgs {
+    int M, N;
+    int chunks;       // blocks per strip of columns
+    int rows;         // rows per block
+    int act, bf16, dy_f32;
+    const void *dy, *z, *u;  // gated: dH, G, U
+    void *dz, *du;           // gated: dG, dU
+    long long lddy, ldz, ldu, lddz, lddu;
+    float *dbias;
+};
+
+// Eight columns of a row, from a 16-bit or fp32 matrix with 16-byte rows.
+__device__ __forceinline__ void load8(const void *base, long long ld, long long row, int col, int N, bool f32,
+                                      bool bf16, float (&v)[8]) {
+    if (col + 8 <= N) {
+        if (f32) {
+            const float *p = static_cast<const float *>(base) + row * ld + col;
+            uint32_t w[8];
+            ld_v4(p, w);
+            ld_v4(p + 4, w + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+        } else {
+            uint32_t w[4];
+            ld_v4(static_cast<const uint16_t *>(base) + row * ld + col, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpack16(w[j], bf16, v[2 * j], v[2 * j + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            v[j] = col + j >= N ? 0.0f
+                   : f32        ? (static_cast<const float *>(base) + row * ld + col)[j]
+                                : from16((static_cast<const uint16_t *>(base) + row * ld + col)[j], bf16);
+    }
+}
+__device__ __forceinline__ void store8(void *base, long long ld, long long row, int col, int N, bool bf16,
+                                       const float (&v)[8]) {
+    uint16_t *p = static_cast<uint16_t *>(base) + row * ld + col;
+    if (col + 8 <= N) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pack16(v[2 * j], v[2 * j + 1], bf16);
+        st_v4(p, w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + j < N) p[j] = to16(v[j], bf16);
+    }
+}
+
+// A block takes `rows` rows of one strip of 64 columns, EW_BATCH x 32 rows at
+// a time: all of a batch's loads are issued before its stores, and an element
+// is stored by the thread that loaded it, so the outputs may lie over the
+// inputs.
+//
+// SUM (dbias): the blocks of a strip are one cluster of at most eight.  Each
+// adds its rows in fp32 registers, then over its 32 row-threads in shared
+// memory; the cluster's first block reads the others' sums and adds them in
+// rank order.  No atomics and no workspace: the result does not depend on
+// timing, and calls may overlap.
+template <bool GATED, bool SUM>
+__global__ void __launch_bounds__(EW_THREADS) act_grad_kernel(const EwArgs p) {
+    __shared__ float part[EW_ROWS][EW_COLS];
+    const int strips = (p.N + EW_COLS - 1) / EW_COLS;
+    // A strip's blocks next to one another for the cluster; else row by row.
+    const int strip = SUM ? static_cast<int>(blockIdx.x / p.chunks) : static_cast<int>(blockIdx.x % strips);
+    const int chunk = SUM ? static_cast<int>(blockIdx.x % p.chunks) : static_cast<int>(blockIdx.x / strips);
+    const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+    const int col = strip * EW_COLS + tx * 8;
+    const long long first = static_cast<long long>(chunk) * p.rows;
+    const long long last = min(first + p.rows, static_cast<long long>(p.M));
+    const bool bf16 = p.bf16 != 0;
+    float sum[8] = {};
+
+    grid_dependency_wait();
+    if (col < p.N) {
+        for (long long r0 = first + ty; r0 < last; r0 += EW_ROWS * EW_BATCH) {
+            float dy[EW_BATCH][8], z[EW_BATCH][8], u[GATED ? EW_BATCH : 1][8];
+#pragma unroll
+            for (int b = 0; b < EW_BATCH; ++b) {
+                const long long r = r0 + b * EW_ROWS;
+                if (r >= last) break;
+                load8(p.dy, p.lddy, r, col, p.N, p.dy_f32, bf16, dy[b]);
+                if (p.z) load8(p.z, p.ldz, r, col, p.N, false, bf16, z[b]);
+                if (GATED) load8(p.u, p.ldu, r, col, p.N, false, bf16, u[GATED ? b : 0]);
+            }
+#pragma unroll
+            for (int b = 0; b < EW_BATCH; ++b) {
+                const long long r = r0 + b * EW_ROWS;
+                if (r >= last) break;
+                if (GATED) {
+                    float dg[8], du[8];
+                    with_act(p.act, [&](auto tag) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            float value, grad;
+                            act_both<decltype(tag)::value>(z[b][j], value, grad);
+                            dg[j] = dy[b][j] * u[GATED ? b : 0][j] * grad;
+                            du[j] = dy[b][j] * value;
+                        }
+                    });
+                    store8(p.dz, p.lddz, r, col, p.N, bf16, dg);
+                    store8(p.du, p.lddu, r, col, p.N, bf16, du);
+                } else {
+                    if (p.act != CUDAIR_ACT_NONE)
+                        with_act(p.act, [&](auto tag) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                float value, grad;
+                                act_both<decltype(tag)::value>(z[b][j], value, grad);
+                                dy[b][j] *= grad;
+                            }
+                        });
+                    if (p.dz) store8(p.dz, p.lddz, r, col, p.N, bf16, dy[b]);
+                    if (SUM) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) sum[j] += dy[b][j];
+                    }
+                }
+            }
+        }
+    }
+    if (SUM) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[ty][tx * 8 + j] = sum[j];
+        __syncthreads();
+        float s = 0.0f;
+        if (threadIdx.x < EW_COLS) {
+#pragma unroll
+            for (int r = 0; r < EW_ROWS; ++r) s += part[r][threadIdx.x];
+            part[0][threadIdx.x] = s;
+        }
+        cluster_sync();
+        if (chunk == 0 && threadIdx.x < EW_COLS) {
+            const uint32_t mine = smem_u32(&part[0][threadIdx.x]);
+            for (int c = 1; c < p.chunks; ++c) {
+                float other;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(mapa_shared(mine, c)) : "memory");
+                s += other;
+            }
+            const int n = strip * EW_COLS + static_cast<int>(threadIdx.x);
+            if (n < p.N) p.dbias[n] = s;
+        }
+        __syncwarp();
+        cluster_sync();  // no block leaves while its sums are being read
+    }
+}
+
+namespace {
+
+int act_grad_launch(EwArgs &p, bool gated, cudaStream_t stream) {
+    const int64_t strips = (static_cast<int64_t>(p.N) + EW_COLS - 1) / EW_COLS;
+    const bool sum = p.dbias != nullptr;
+    const int64_t step = EW_ROWS * EW_BATCH;
+    const int64_t steps = (static_cast<int64_t>(p.M) + step - 1) / step;
+    // With a sum, at most eight blocks (a portable cluster) share a strip.
+    const int64_t chunks = sum ? (steps < 1 ? 1 : steps < 8 ? steps : 8) : steps;
+    p.chunks = static_cast<int>(chunks);
+    p.rows = static_cast<int>((steps + chunks - 1) / chunks * step);
+    if (strips * chunks > INT32_MAX)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: linear: M=%d x N=%d is too large", p.M, p.N);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(chunks);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(strips * chunks), 1, 1);
+    cfg.blockDim = dim3(EW_THREADS, 1, 1);
+    cfg.stream = stream;
+    cfg.attrs = gemm_pdl_mode() > 0 ? attr : attr + 1;
+    cfg.numAttrs = (gemm_pdl_mode() > 0 ? 1 : 0) + (sum ? 1 : 0);
+    const cudaError_t e = gated ? cudaLaunchKernelEx(&cfg, act_grad_kernel<true, false>, p)
+                          : sum ? cudaLaunchKernelEx(&cfg, act_grad_kernel<false, true>, p)
+                                : cudaLaunchKernelEx(&cfg, act_grad_kernel<false, false>, p);
+    return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "act_grad_kernel launch");
+}
+
+// ---- argument rules ------------------------------------------------------------------
+
+constexpr int64_t kMaxSize = INT32_MAX - 1024;  // tile arithmetic is 32-bit
+
+int check_sizes(const char *op, int64_t M, int64_t N, int64_t K) {
+    if (M < 0 || N < 0 || K < 0)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: negative size M=%lld N=%lld K=%lld", op, (long long)M,
+                         (long long)N, (long long)K);
+    if (M > kMaxSize || N > kMaxSize || K > kMaxSize)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: sizes must be at most %lld", op, (long long)kMaxSize);
+    return CUDAIR_OK;
+}
+
+int check_flags(const char *op, uint32_t flags, uint32_t known, uint32_t act) {
+    if (flags & ~known) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: unknown flags 0x%x", op, flags & ~known);
+    if (act > CUDAIR_ACT_SILU)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: unknown activation %u", op, act);
+    return CUDAIR_OK;
+}
+
+// A rows x cols matrix: present, 16-byte aligned, rows of whole 16 bytes.
+int check_mat(const char *op, const char *name, const void *p, int64_t ld, int64_t cols, int elem) {
+    if (!p) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: nil pointer (%s)", op, name);
+    if (reinterpret_cast<uintptr_t>(p) & 15u)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: %s must be 16-byte aligned", op, name);
+    if (ld < cols)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: pitch %lld of %s is below its %lld columns", op,
+                         (long long)ld, name, (long long)cols);
+    if (ld % (16 / elem))
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: pitch %lld of %s must be a multiple of %d (16-byte rows)",
+                         op, (long long)ld, name, 16 / elem);
+    if (ld > (INT64_MAX >> 34))  // row * pitch stays far inside 64 bits
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: pitch %lld of %s is too large", op, (long long)ld, name);
+    return CUDAIR_OK;
+}
+
+#define CUDAIR_TRY(call)                        \
+    do {                                        \
+        const int rc_ = (call);                 \
+        if (rc_ != CUDAIR_OK) return rc_;       \
+    } while (0)
+
+Operand operand(const void *p, int64_t ld, bool mn) {
+    Operand o;
+    o.p = p;
+    o.ld = ld;
+    o.mn = mn;
+    return o;
+}
+OutMat out_mat(void *p, int64_t ld, bool f32) {
+    OutMat m;
+    m.p = p;
+    m.ld = ld;
+    m.f32 = f32;
+    return m;
+}
+
+}  // namespace
+
+int product_launch(const Product &p, cudaStream_t stream) {
+    int sms = 0;
+    unsigned int *status = nullptr;
+    CUDAIR_TRY(sm_count_current_device(&sms));
+    CUDAIR_TRY(wait_status_current_device(&status));
+    return product_pair_launch(p, sms, status, stream);
+}
+
+}  // namespace ffn
+}  // namespace cudair
+
+using namespace cudair;
+using namespace cudair::ffn;
+
+CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
+    clear_error();
+    const char *op = "linear";
+    if (!q) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: nil arguments", op);
+    CUDAIR_TRY(check_flags(op, q->flags,
+                           CUDAIR_GEMM_BF16 | CUDAIR_GEMM_B_T | CUDAIR_LINEAR_D_F32 | CUDAIR_LINEAR_BIAS_16,
+                           q->act));
+    CUDAIR_TRY(check_sizes(op, q->M, q->N, q->K));
+    if (q->M == 0 || q->N == 0) return CUDAIR_OK;
+    const bool bt = q->flags & CUDAIR_GEMM_B_T, d_f32 = q->flags & CUDAIR_LINEAR_D_F32;
+    const bool bias16 = q->flags & CUDAIR_LINEAR_BIAS_16;
+    if (q->K > 0) {
+        CUDAIR_TRY(check_mat(op, "a", q->a, q->lda, q->K, 2));
+        CUDAIR_TRY(check_mat(op, "b", q->b, q->ldb, bt ? q->K : q->N, 2));
+    }
+    CUDAIR_TRY(check_mat(op, "d", q->d, q->ldd, q->N, d_f32 ? 4 : 2));
+    if (q->residual) CUDAIR_TRY(check_mat(op, "residual", q->residual, q->ldres, q->N, d_f32 ? 4 : 2));
+    if (q->z) CUDAIR_TRY(check_mat(op, "z", q->z, q->ldz, q->N, 2));
+    if (q->bias && (reinterpret_cast<uintptr_t>(q->bias) & (bias16 ? 1u : 3u)))
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: bias must be aligned to its elements", op);
+    if (q->residual == q->d && q->residual && q->ldres != q->ldd)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a residual in D's memory needs D's pitch", op);
+    Product p;
+    p.M = q->M;
+    p.N = q->N;
+    p.K = q->K;
+    p.a[0] = operand(q->a, q->lda, false);
+    p.b[0] = operand(q->b, q->ldb, !bt);
+    p.d[0] = out_mat(q->d, q->ldd, d_f32);
+    p.z[0] = out_mat(q->z, q->ldz, false);
+    p.residual = out_mat(const_cast<void *>(q->residual), q->ldres, d_f32);
+    p.bias = q->bias;
+    p.bias16 = bias16;
+    p.act = static_cast<int>(q->act);
+    p.bf16 = q->flags & CUDAIR_GEMM_BF16;
+    return product_launch(p, static_cast<cudaStream_t>(stream));
+}
+
+CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
+    clear_error();
+    const char *op = "gated";
+    if (!q) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: nil arguments", op);
+    CUDAIR_TRY(check_flags(op, q->flags, CUDAIR_GEMM_BF16 | CUDAIR_GEMM_B_T, q->act));
+    CUDAIR_TRY(check_sizes(op, q->M, q->N, q->K));
+    if (q->M == 0 || q->N == 0) return CUDAIR_OK;
+    const bool bt = q->flags & CUDAIR_GEMM_B_T;
+    if (q->K > 0) {
+        CUDAIR_TRY(check_mat(op, "x", q->x, q->ldx, q->K, 2));
+        CUDAIR_TRY(check_mat(op, "wg", q->wg, q->ldwg, bt ? q->K : q->N, 2));
+        CUDAIR_TRY(check_mat(op, "wu", q->wu, q->ldwu, bt ? q->K : q->N, 2));
+    }
+    CUDAIR_TRY(check_mat(op, "h", q->h, q->ldh, q->N, 2));
+    if (!q->g != !q->u) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: g and u are given together", op);
+    if (q->g) {
+        CUDAIR_TRY(check_mat(op, "g", q->g, q->ldg, q->N, 2));
+        CUDAIR_TRY(check_mat(op, "u", q->u, q->ldu, q->N, 2));
+    }
+    Product p;
+    p.form = Form::gated;
+    p.M = q->M;
+    p.N = q->N;
+    p.K = q->K;
+    p.a[0] = operand(q->x, q->ldx, false);
+    p.b[0] = operand(q->wg, q->ldwg, !bt);
+    p.b[1] = operand(q->wu, q->ldwu, !bt);
+    p.d[0] = out_mat(q->h, q->ldh, false);
+    p.z[0] = out_mat(q->g, q->ldg, false);
+    p.z[1] = out_mat(q->u, q->ldu, false);
+    p.act = static_cast<int>(q->act);
+    p.bf16 = q->flags & CUDAIR_GEMM_BF16;
+    return product_launch(p, static_cast<cudaStream_t>(stream));
+}
+
+CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void *stream) {
+    clear_error();
+    const char *op = "linear_backward";
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!q) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: nil arguments", op);
+    CUDAIR_TRY(check_flags(op, q->flags,
+                           CUDAIR_GEMM_BF16 | CUDAIR_GEMM_B_T | CUDAIR_LINEAR_D_F32 | CUDAIR_LINEAR_DA_F32 |
+                               CUDAIR_LINEAR_DB_F32,
+                           q->act));
+    CUDAIR_TRY(check_sizes(op, q->M, q->N, q->K));
+    const bool bt = q->flags & CUDAIR_GEMM_B_T, dy_f32 = q->flags & CUDAIR_LINEAR_D_F32;
+    const bool bf16 = q->flags & CUDAIR_GEMM_BF16, has_act = q->act != CUDAIR_ACT_NONE;
+    const bool da_f32 = q->flags & CUDAIR_LINEAR_DA_F32, db_f32 = q->flags & CUDAIR_LINEAR_DB_F32;
+    const bool own_dz = has_act || dy_f32;
+    if (!own_dz && q->dz)
+        return set_error(CUDAIR_ERR_INVALID,
+                         "cudair: %s: without an activation a 16-bit dY is dZ itself: dz must be nil", op);
+    if (q->M > 0 && q->N > 0) {
+        CUDAIR_TRY(check_mat(op, "dy", q->dy, q->lddy, q->N, dy_f32 ? 4 : 2));
+        if (has_act) CUDAIR_TRY(check_mat(op, "z", q->z, q->ldz, q->N, 2));
+        if (own_dz) {
+            CUDAIR_TRY(check_mat(op, "dz", q->dz, q->lddz, q->N, 2));
+            if (q->dz == q->dy && (dy_f32 || q->lddz != q->lddy))
+                return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dz in dY's memory needs its type and pitch", op);
+            if (q->dz == q->z && has_act && q->lddz != q->ldz)
+                return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dz in z's memory needs its pitch", op);
+        }
+    }
+    const bool want_da = q->da && q->M > 0 && q->K > 0, want_db = q->db && q->N > 0 && q->K > 0;
+    if (want_da) {
+        CUDAIR_TRY(check_mat(op, "da", q->da, q->ldda, q->K, da_f32 ? 4 : 2));
+        if (q->N > 0) CUDAIR_TRY(check_mat(op, "b", q->b, q->ldb, bt ? q->K : q->N, 2));
+    }
+    if (want_db) {
+        CUDAIR_TRY(check_mat(op, "db", q->db, q->lddb, bt ? q->K : q->N, db_f32 ? 4 : 2));
+        if (q->M > 0) CUDAIR_TRY(check_mat(op, "a", q->a, q->lda, q->K, 2));
+    }
+    if (q->dbias && (reinterpret_cast<uintptr_t>(q->dbias) & 3u))
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dbias must be 4-byte aligned", op);
+
+    int sms = 0;
+    CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
+    // dZ, and the bias's gradient from it (M = 0: its empty sums).
+    const bool elementwise = q->N > 0 && ((own_dz && q->M > 0) || q->dbias);
+    if (elementwise) {
+        EwArgs e = {};
+        e.M = static_cast<int>(q->M);
+        e.N = static_cast<int>(q->N);
+        e.act = static_cast<int>(q->act);
+        e.bf16 = bf16;
+        e.dy_f32 = dy_f32;
+        e.dy = q->dy;
+        e.z = has_act ? q->z : nullptr;
+        e.dz = own_dz ? q->dz : nullptr;
+        e.lddy = q->lddy;
+        e.ldz = q->ldz;
+        e.lddz = q->lddz;
+        e.dbias = q->dbias;
+        CUDAIR_TRY(act_grad_launch(e, false, s));
+    }
+    const void *dz = own_dz ? q->dz : q->dy;
+    const int64_t lddz = own_dz ? q->lddz : q->lddy;
+    if (want_da) {
+        Product p;
+        p.M = q->M;
+        p.N = q->K;
+        p.K = q->N;
+        p.a[0] = operand(dz, lddz, false);
+        p.b[0] = operand(q->b, q->ldb, bt);  // the contraction runs over N
+        p.d[0] = out_mat(q->da, q->ldda, da_f32);
+        p.bf16 = bf16;
+        CUDAIR_TRY(product_launch(p, s));
+    }
+    if (want_db) {
+        Product p;
+        p.M = bt ? q->N : q->K;
+        p.N = bt ? q->K : q->N;
+        p.K = q->M;
+        const Operand x = operand(q->a, q->lda, true), g = operand(dz, lddz, true);
+        p.a[0] = bt ? g : x;
+        p.b[0] = bt ? x : g;
+        p.d[0] = out_mat(q->db, q->lddb, db_f32);
+        p.bf16 = bf16;
+        CUDAIR_TRY(product_launch(p, s));
+    }
+    return CUDAIR_OK;
+}
+
+CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *stream) {
+    clear_error();
+    const char *op = "gated_backward";
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!q) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: nil arguments", op);
+    CUDAIR_TRY(check_flags(op, q->flags,
+                           CUDAIR_GEMM_BF16 | CUDAIR_GEMM_B_T | CUDAIR_LINEAR_DA_F32 | CUDAIR_LINEAR_DB_F32,
+                           q->act));
+    CUDAIR_TRY(check_sizes(op, q->M, q->N, q->K));
+    const bool bt = q->flags & CUDAIR_GEMM_B_T, bf16 = q->flags & CUDAIR_GEMM_BF16;
+    const bool dx_f32 = q->flags & CUDAIR_LINEAR_DA_F32, dw_f32 = q->flags & CUDAIR_LINEAR_DB_F32;
+    if (!q->dwg != !q->dwu)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dwg and dwu are given together", op);
+    if (q->M > 0 && q->N > 0) {
+        CUDAIR_TRY(check_mat(op, "dh", q->dh, q->lddh, q->N, 2));
+        CUDAIR_TRY(check_mat(op, "g", q->g, q->ldg, q->N, 2));
+        CUDAIR_TRY(check_mat(op, "u", q->u, q->ldu, q->N, 2));
+        CUDAIR_TRY(check_mat(op, "dg", q->dg, q->lddg, q->N, 2));
+        CUDAIR_TRY(check_mat(op, "du", q->du, q->lddu, q->N, 2));
+        if (q->dg == q->du) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dg and du share memory", op);
+        const struct {
+            const void *p;
+            int64_t ld;
+        } in[3] = {{q->dh, q->lddh}, {q->g, q->ldg}, {q->u, q->ldu}};
+        for (const auto &m : in)
+            if ((m.p == q->dg && m.ld != q->lddg) || (m.p == q->du && m.ld != q->lddu))
+                return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dg or du in an input's memory needs its pitch",
+                                 op);
+    }
+    const bool want_dx = q->dx && q->M > 0 && q->K > 0, want_dw = q->dwg && q->N > 0 && q->K > 0;
+    const int64_t wcols = bt ? q->K : q->N;
+    if (want_dx) {
+        CUDAIR_TRY(check_mat(op, "dx", q->dx, q->lddx, q->K, dx_f32 ? 4 : 2));
+        if (q->N > 0) {
+            CUDAIR_TRY(check_mat(op, "wg", q->wg, q->ldwg, wcols, 2));
+            CUDAIR_TRY(check_mat(op, "wu", q->wu, q->ldwu, wcols, 2));
+        }
+    }
+    if (want_dw) {
+        CUDAIR_TRY(check_mat(op, "dwg", q->dwg, q->lddwg, wcols, dw_f32 ? 4 : 2));
+        CUDAIR_TRY(check_mat(op, "dwu", q->dwu, q->lddwu, wcols, dw_f32 ? 4 : 2));
+        if (q->M > 0) CUDAIR_TRY(check_mat(op, "x", q->x, q->ldx, q->K, 2));
+    }
+    int sms = 0;
+    CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
+    if (q->M > 0 && q->N > 0) {
+        EwArgs e = {};
+        e.M = static_cast<int>(q->M);
+        e.N = static_cast<int>(q->N);
+        e.act = static_cast<int>(q->act);
+        e.bf16 = bf16;
+        e.dy = q->dh;
+        e.z = q->g;
+        e.u = q->u;
+        e.dz = q->dg;
+        e.du = q->du;
+        e.lddy = q->lddh;
+        e.ldz = q->ldg;
+        e.ldu = q->ldu;
+        e.lddz = q->lddg;
+        e.lddu = q->lddu;
+        CUDAIR_TRY(act_grad_launch(e, true, s));
+    }
+    if (want_dx) {
+        Product p;
+        p.form = Form::sum;
+        p.M = q->M;
+        p.N = q->K;
+        p.K = q->N;
+        p.a[0] = operand(q->dg, q->lddg, false);
+        p.a[1] = operand(q->du, q->lddu, false);
+        p.b[0] = operand(q->wg, q->ldwg, bt);
+        p.b[1] = operand(q->wu, q->ldwu, bt);
+        p.d[0] = out_mat(q->dx, q->lddx, dx_f32);
+        p.bf16 = bf16;
+        CUDAIR_TRY(product_launch(p, s));
+    }
+    if (want_dw) {
+        Product p;
+        p.form = Form::pair;
+        p.M = bt ? q->N : q->K;
+        p.N = bt ? q->K : q->N;
+        p.K = q->M;
+        const Operand x = operand(q->x, q->ldx, true);
+        const Operand dg = operand(q->dg, q->lddg, true), du = operand(q->du, q->lddu, true);
+        p.a[0] = bt ? dg : x;
+        p.a[1] = bt ? du : x;
+        p.b[0] = bt ? x : dg;
+        p.b[1] = bt ? x : du;
+        p.d[0] = out_mat(q->dwg, q->lddwg, dw_f32);
+        p.d[1] = out_mat(q->dwu, q->lddwu, dw_f32);
+        p.bf16 = bf16;
+        CUDAIR_TRY(product_launch(p, s));
+    }
+    return CUDAIR_OK;
+}

@@ -1,0 +1,238 @@
+// linear_epilogue.cuh - what the linear and gated kernels do with an
+// accumulator: the activations and their derivatives, and the loads and stores
+// of a row's 32 consecutive columns in 16 or 32 bits.
+//
+// Everything is computed in fp32 and rounded once, to nearest, when it is
+// stored.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "../../include/cudair_b200.h"
+
+namespace cudair {
+namespace ffn {
+
+// ---- activations ---------------------------------------------------------------
+//
+//   relu       max(z, 0), a NaN kept
+//   silu       z s(z), s(z) = 1 / (1 + e^-z)
+//   gelu       z P(z), P the normal distribution's integral (normcdff keeps
+//              its relative precision for negative z, where 1 + erf cancels)
+//   gelu_tanh  z (1 + tanh(y)) / 2 with y = sqrt(2/pi) (z + 0.044715 z^3),
+//              computed as z s(2y), which is the same and does not cancel
+
+constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluB = 0.044715f;
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float z) {
+    if (ACT == CUDAIR_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if (ACT == CUDAIR_ACT_SILU) return z * sigmoid(z);
+    if (ACT == CUDAIR_ACT_GELU) return z * normcdff(z);
+    if (ACT == CUDAIR_ACT_GELU_TANH) return z * sigmoid(kGeluC * (z + kGeluB * z * z * z));
+    return z;
+}
+
+// The value and the derivative at z.
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float &value, float &grad) {
+    if (ACT == CUDAIR_ACT_RELU) {
+        value = z < 0.0f ? 0.0f : z;
+        grad = z <= 0.0f ? 0.0f : 1.0f;
+    } else if (ACT == CUDAIR_ACT_SILU) {
+        const float s = sigmoid(z);
+        value = z * s;
+        grad = s * (1.0f + z * (1.0f - s));
+    } else if (ACT == CUDAIR_ACT_GELU) {
+        const float p = normcdff(z);
+        value = z * p;
+        grad = p + z * (0.3989422804014327f * expf(-0.5f * z * z));
+    } else if (ACT == CUDAIR_ACT_GELU_TANH) {
+        const float z2 = z * z;
+        const float s = sigmoid(kGeluC * (z + kGeluB * z * z2));
+        value = z * s;
+        // s (1 - s) is zero where s is 0 or 1; z^2 may be infinite there.
+        const float w = s * (1.0f - s);
+        grad = w == 0.0f ? s : s + z * w * (kGeluC * (1.0f + 3.0f * kGeluB * z2));
+    } else {
+        value = z;
+        grad = 1.0f;
+    }
+}
+
+// Calls f with the activation as a compile-time constant: the choice is made
+// once per block of elements, not per element.
+template <int V>
+struct ActTag {
+    static constexpr int value = V;
+};
+template <class F>
+__device__ __forceinline__ void with_act(int act, F &&f) {
+    switch (act) {
+        case CUDAIR_ACT_RELU: f(ActTag<CUDAIR_ACT_RELU>{}); break;
+        case CUDAIR_ACT_GELU: f(ActTag<CUDAIR_ACT_GELU>{}); break;
+        case CUDAIR_ACT_GELU_TANH: f(ActTag<CUDAIR_ACT_GELU_TANH>{}); break;
+        case CUDAIR_ACT_SILU: f(ActTag<CUDAIR_ACT_SILU>{}); break;
+        default: f(ActTag<CUDAIR_ACT_NONE>{}); break;
+    }
+}
+
+// ---- 16-bit conversions ----------------------------------------------------------
+
+__device__ __forceinline__ float from16(uint16_t h, bool bf16) {
+    return bf16 ? __uint_as_float(static_cast<uint32_t>(h) << 16) : __half2float(__ushort_as_half(h));
+}
+__device__ __forceinline__ uint16_t to16(float f, bool bf16) {
+    return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(f)) : __half_as_ushort(__float2half_rn(f));
+}
+__device__ __forceinline__ void unpack16(uint32_t w, bool bf16, float &lo, float &hi) {
+    if (bf16) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xFFFF0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        lo = f.x;
+        hi = f.y;
+    }
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// ---- global memory, 32 or 16 bytes at a time ----------------------------------------
+
+__device__ __forceinline__ void st_v8(void *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ void st_v4(void *p, const uint32_t *w) {
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3])
+                 : "memory");
+}
+__device__ __forceinline__ void ld_v8(const void *p, uint32_t *w) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]),
+                   "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void ld_v4(const void *p, uint32_t *w) {
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "l"(p)
+                 : "memory");
+}
+
+// A row-major matrix that an epilogue reads or writes.
+struct Mat {
+    void *p;        // nullptr: absent
+    long long ld;   // elements
+    int f32;        // 32-bit elements, else 16-bit of the operands' type
+    int wide;       // base and pitch are multiples of 32 bytes, else of 16
+};
+
+// One row's 32 columns from col (a multiple of 32, below N): whole 32-byte
+// sectors where the matrix allows it, else 16 bytes at a time; the columns of
+// a last block that ends inside it one by one, none beyond N touched.
+__device__ __forceinline__ void store_row32(const Mat &m, long long row, int col, int N, bool bf16,
+                                            const float (&v)[32]) {
+    if (m.f32) {
+        float *p = static_cast<float *>(m.p) + row * m.ld + col;
+        if (col + 32 <= N) {
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(v[j]);
+            if (m.wide) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) st_v8(p + 8 * j, w + 8 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) st_v4(p + 4 * j, w + 4 * j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < N) p[j] = v[j];
+        }
+    } else {
+        uint16_t *p = static_cast<uint16_t *>(m.p) + row * m.ld + col;
+        if (col + 32 <= N) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack16(v[2 * j], v[2 * j + 1], bf16);
+            if (m.wide) {
+                st_v8(p, w);
+                st_v8(p + 16, w + 8);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) st_v4(p + 8 * j, w + 4 * j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < N) p[j] = to16(v[j], bf16);
+        }
+    }
+}
+
+// Adds one row's 32 columns to v.
+__device__ __forceinline__ void add_row32(const Mat &m, long long row, int col, int N, bool bf16,
+                                          float (&v)[32]) {
+    if (m.f32) {
+        const float *p = static_cast<const float *>(m.p) + row * m.ld + col;
+        if (col + 32 <= N) {
+            uint32_t w[32];
+            if (m.wide) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ld_v8(p + 8 * j, w + 8 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ld_v4(p + 4 * j, w + 4 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(w[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < N) v[j] += p[j];
+        }
+    } else {
+        const uint16_t *p = static_cast<const uint16_t *>(m.p) + row * m.ld + col;
+        if (col + 32 <= N) {
+            uint32_t w[16];
+            if (m.wide) {
+                ld_v8(p, w);
+                ld_v8(p + 16, w + 8);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ld_v4(p + 8 * j, w + 4 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                float lo, hi;
+                unpack16(w[j], bf16, lo, hi);
+                v[2 * j] += lo;
+                v[2 * j + 1] += hi;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col + j < N) v[j] += from16(p[j], bf16);
+        }
+    }
+}
+
+}  // namespace ffn
+}  // namespace cudair

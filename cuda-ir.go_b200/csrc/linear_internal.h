@@ -1,0 +1,52 @@
+// linear_internal.h - one product of the feed-forward operators, as their
+// entry points describe it to the kernels that run it.
+#pragma once
+
+#include "cudair_internal.h"
+
+namespace cudair {
+namespace ffn {
+
+// A 16-bit operand: `rows` rows of the product (of A) or columns (of B) by
+// `depth` of the contraction.  As stored, either the contraction runs along
+// memory (mn false) or the rows do (mn true).
+struct Operand {
+    const void *p = nullptr;
+    int64_t ld = 0;
+    bool mn = false;
+};
+
+// D[i] = epilogue(A[i] . B[i]) for one or two problems of one shape:
+//   plain    one problem
+//   pair     two independent problems (the gradients of two weights)
+//   sum      D[0] = epilogue(A[0].B[0] + A[1].B[1]) (the gradient of X)
+//   gated    D[0] = act(A[0].B[0]) * (A[0].B[1])
+enum class Form { plain, pair, sum, gated };
+
+struct OutMat {
+    void *p = nullptr;
+    int64_t ld = 0;
+    bool f32 = false;
+};
+
+struct Product {
+    Form form = Form::plain;
+    int64_t M = 0, N = 0, K = 0;
+    Operand a[2], b[2];
+    OutMat d[2];
+    const void *bias = nullptr;  // N values (plain form)
+    bool bias16 = false;
+    OutMat residual;             // plain form
+    OutMat z[2];                 // plain: Z in z[0]; gated: G and U
+    int act = CUDAIR_ACT_NONE;
+    bool bf16 = false;
+};
+
+// Runs the product on the current device: M and N positive, K >= 0.
+int product_launch(const Product &p, cudaStream_t stream);
+
+// The persistent CTA-pair kernel (linear_sm100.cu).
+int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cudaStream_t stream);
+
+}  // namespace ffn
+}  // namespace cudair

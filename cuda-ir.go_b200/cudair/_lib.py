@@ -45,6 +45,10 @@ SIGNATURES = {
                                    c_vp]),
     "cudair_gemm": (c_int, [c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                             c_u32, c_vp]),
+    "cudair_linear": (c_int, [c_vp, c_vp]),
+    "cudair_linear_backward": (c_int, [c_vp, c_vp]),
+    "cudair_gated": (c_int, [c_vp, c_vp]),
+    "cudair_gated_backward": (c_int, [c_vp, c_vp]),
     "cudair_set_gemm_variant": (c_int, [c_int]),
     "cudair_set_gemm_pdl": (c_int, [c_int]),
     "cudair_vecadd": (c_int, [c_vp, c_vp, c_vp, ctypes.c_int32, c_vp]),
@@ -60,6 +64,22 @@ SIGNATURES = {
     "cudair_ipc_close": (c_int, [c_vp]),
     "cudair_peer_copy": (c_int, [c_vp, c_vp, c_size, c_vp]),
 }
+
+
+
+def _struct(name, pointers, sizes):
+    """The argument structs of include/cudair_b200.h: pointers, 64-bit sizes
+    and pitches, then act and flags."""
+    fields = [(f, c_vp) for f in pointers.split()] + [(f, c_i64) for f in sizes.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields + [("act", c_u32), ("flags", c_u32)]})
+
+
+LinearArgs = _struct("cudair_linear_args", "a b bias residual d z", "M N K lda ldb ldres ldd ldz")
+LinearBackwardArgs = _struct("cudair_linear_backward_args", "dy a b z dz da db dbias",
+                             "M N K lddy lda ldb ldz lddz ldda lddb")
+GatedArgs = _struct("cudair_gated_args", "x wg wu h g u", "M N K ldx ldwg ldwu ldh ldg ldu")
+GatedBackwardArgs = _struct("cudair_gated_backward_args", "dh x wg wu g u dg du dx dwg dwu",
+                            "M N K lddh ldx ldwg ldwu ldg ldu lddg lddu lddx lddwg lddwu")
 
 # Error codes of include/cudair_b200.h.
 OK, ERR_INVALID, ERR_DRIVER, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED = range(6)

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 
-from ._lib import CudairError, check, lib
+from ._lib import (CudairError, GatedArgs, GatedBackwardArgs, LinearArgs, LinearBackwardArgs, check, lib)
 
 
 def _stream(stream):
@@ -95,6 +95,189 @@ def gemm_ex(a, b, c, bias=None, b_trans=False, overwrite=False, stream=None) -> 
         bias_ptr, ldbias = bias.data_ptr(), bias.stride(0)
     check(lib().cudair_gemm(a.data_ptr(), b.data_ptr(), c.data_ptr(), bias_ptr, M, N, K, a.stride(0),
                             b.stride(0), c.stride(0), ldbias, flags, _stream(stream)))
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+LINEAR_D_F32, LINEAR_BIAS_16, LINEAR_DA_F32, LINEAR_DB_F32 = 0x10, 0x20, 0x40, 0x80
+
+
+def _act(op, act):
+    try:
+        return ACTIVATIONS[act]
+    except (KeyError, TypeError):
+        raise CudairError(1, f"cudair: {op}: act must be one of {', '.join(ACTIVATIONS)}, got {act!r}") from None
+
+
+def _type(op, t, name):
+    """The 16-bit type of an operation's operands, from its first one."""
+    import torch
+    dt = getattr(t, "dtype", None)
+    if dt is not torch.float16 and dt is not torch.bfloat16:
+        raise CudairError(1, f"cudair: {op}: {name} must be a float16 or bfloat16 tensor, got {dt}")
+    return dt
+
+
+def _mat(op, name, t, dtypes, rows, cols, device):
+    """Checks a rows x cols matrix and returns its pointer and row pitch."""
+    if not getattr(t, "is_cuda", False):
+        raise CudairError(1, f"cudair: {op}: {name} must be a CUDA tensor")
+    if t.dtype not in dtypes:
+        raise CudairError(1, f"cudair: {op}: {name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if t.get_device() != device:
+        raise CudairError(1, f"cudair: {op}: {name} is on {t.device}, the current device is cuda:{device}")
+    if t.shape != (rows, cols):
+        raise CudairError(1, f"cudair: {op}: {name} must be {rows} x {cols}, got {tuple(t.shape)}")
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
+        raise CudairError(1, f"cudair: {op}: {name} needs unit inner stride")
+    # One row has no pitch of its own, and an empty matrix no rows.
+    return t.data_ptr(), -(-cols // 8) * 8 if rows <= 1 or cols == 0 else ld
+
+
+def _device():
+    import torch
+    return torch.cuda.current_device()
+
+
+def _dims(op, x, xname, w, wname, b_trans):
+    """(M, N, K) of x (M x K) and a weight (K x N, or N x K with b_trans)."""
+    if x.dim() != 2 or w.dim() != 2:
+        raise CudairError(1, f"cudair: {op}: {xname} and {wname} must be matrices")
+    return x.shape[0], w.shape[0 if b_trans else 1], x.shape[1]
+
+
+def linear(a, b, d, bias=None, residual=None, z=None, act="none", b_trans=False, stream=None) -> None:
+    """d = act(a @ B + bias) + residual with B = b (K x N), or b.T when b_trans
+    (b is N x K): one kernel (cudair_linear).  a and b are both fp16 or both
+    bf16; d is of their type or fp32; bias has N values (fp32 or a's type);
+    residual is M x N of d's type and may be d itself; z (M x N of a's type)
+    receives a @ B + bias for linear_backward.  act: "none", "relu", "gelu",
+    "gelu_tanh" or "silu".  Rows start on 16 bytes."""
+    import torch
+    op, dev = "linear", _device()
+    dt = _type(op, a, "a")
+    M, N, K = _dims(op, a, "a", b, "b", b_trans)
+    t16, flags = (dt,), (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
+    pa, lda = _mat(op, "a", a, t16, M, K, dev)
+    pb, ldb = _mat(op, "b", b, t16, N if b_trans else K, K if b_trans else N, dev)
+    pd, ldd = _mat(op, "d", d, (dt, torch.float32), M, N, dev)
+    if d.dtype is torch.float32:
+        flags |= LINEAR_D_F32
+    pbias, pres, ldres, pz, ldz = None, None, 0, None, 0
+    if bias is not None:
+        if bias.shape != (N,) or (N > 1 and bias.stride(0) != 1):
+            raise CudairError(1, f"cudair: {op}: bias must have {N} consecutive values")
+        pbias = _mat(op, "bias", bias.view(1, N), (torch.float32, dt), 1, N, dev)[0]
+        if bias.dtype is not torch.float32:
+            flags |= LINEAR_BIAS_16
+    if residual is not None:
+        pres, ldres = _mat(op, "residual", residual, (d.dtype,), M, N, dev)
+    if z is not None:
+        pz, ldz = _mat(op, "z", z, t16, M, N, dev)
+    check(lib().cudair_linear(ctypes.byref(LinearArgs(
+        pa, pb, pbias, pres, pd, pz, M, N, K, lda, ldb, ldres, ldd, ldz, _act(op, act), flags)), _stream(stream)))
+
+
+def linear_backward(dy, a, b, z=None, dz=None, da=None, db=None, dbias=None, act="none", b_trans=False,
+                    stream=None) -> None:
+    """The gradients of linear (cudair_linear_backward), each written where
+    given: da = dz @ B.T (M x K), db = a.T @ dz (stored as b is), dbias (N
+    fp32 values) = dz summed over its rows, with dz = dy * act'(z).  dy is of
+    a's type or fp32 (the gradient of d, and so the residual's).  z (as linear
+    stored it) is needed with an activation; dz (M x N of a's type) with an
+    activation or an fp32 dy, and only then; it may be z's or dy's memory.
+    da and db are of a's type or fp32."""
+    import torch
+    op, dev = "linear_backward", _device()
+    dt = _type(op, a, "a")
+    M, N, K = _dims(op, a, "a", b, "b", b_trans)
+    t16, either = (dt,), (dt, torch.float32)
+    w = (N, K) if b_trans else (K, N)
+    flags = (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
+    pdy, lddy = _mat(op, "dy", dy, either, M, N, dev)
+    if dy.dtype is torch.float32:
+        flags |= LINEAR_D_F32
+    pa, lda = _mat(op, "a", a, t16, M, K, dev)
+    pb, ldb = _mat(op, "b", b, t16, *w, dev)
+    pz = pdz = pda = pdb = pdbias = None
+    ldz = lddz = ldda = lddb = 0
+    if z is not None:
+        pz, ldz = _mat(op, "z", z, t16, M, N, dev)
+    if dz is not None:
+        pdz, lddz = _mat(op, "dz", dz, t16, M, N, dev)
+    if da is not None:
+        pda, ldda = _mat(op, "da", da, either, M, K, dev)
+        flags |= LINEAR_DA_F32 if da.dtype is torch.float32 else 0
+    if db is not None:
+        pdb, lddb = _mat(op, "db", db, either, *w, dev)
+        flags |= LINEAR_DB_F32 if db.dtype is torch.float32 else 0
+    if dbias is not None:
+        if dbias.shape != (N,) or (N > 1 and dbias.stride(0) != 1):
+            raise CudairError(1, f"cudair: {op}: dbias must have {N} consecutive values")
+        pdbias = _mat(op, "dbias", dbias.view(1, N), (torch.float32,), 1, N, dev)[0]
+    check(lib().cudair_linear_backward(ctypes.byref(LinearBackwardArgs(
+        pdy, pa, pb, pz, pdz, pda, pdb, pdbias, M, N, K, lddy, lda, ldb, ldz, lddz, ldda, lddb, _act(op, act),
+        flags)), _stream(stream)))
+
+
+def gated(x, wg, wu, h, g=None, u=None, act="silu", b_trans=False, stream=None) -> None:
+    """h = act(x @ Wg) * (x @ Wu) in one kernel (cudair_gated), with Wg = wg
+    and Wu = wu (K x N), or their transposes when b_trans (both N x K).  All
+    fp16 or all bf16; g and u (both or neither, M x N) receive the two products for
+    gated_backward.  The weights may be halves of one tensor."""
+    import torch
+    op, dev = "gated", _device()
+    dt = _type(op, x, "x")
+    M, N, K = _dims(op, x, "x", wg, "wg", b_trans)
+    t16 = (dt,)
+    w = (N, K) if b_trans else (K, N)
+    flags = (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
+    px, ldx = _mat(op, "x", x, t16, M, K, dev)
+    pwg, ldwg = _mat(op, "wg", wg, t16, *w, dev)
+    pwu, ldwu = _mat(op, "wu", wu, t16, *w, dev)
+    ph, ldh = _mat(op, "h", h, t16, M, N, dev)
+    pg, ldg = (None, 0) if g is None else _mat(op, "g", g, t16, M, N, dev)
+    pu, ldu = (None, 0) if u is None else _mat(op, "u", u, t16, M, N, dev)
+    check(lib().cudair_gated(ctypes.byref(GatedArgs(
+        px, pwg, pwu, ph, pg, pu, M, N, K, ldx, ldwg, ldwu, ldh, ldg, ldu, _act(op, act), flags)),
+        _stream(stream)))
+
+
+def gated_backward(dh, x, wg, wu, g, u, dg, du, dx=None, dwg=None, dwu=None, act="silu", b_trans=False,
+                   stream=None) -> None:
+    """The gradients of gated (cudair_gated_backward): dg = dh * u * act'(g)
+    and du = dh * act(g) (M x N; they may be g's and u's memory), then, where
+    given, dx = dg @ Wg.T + du @ Wu.T and dwg = x.T @ dg, dwu = x.T @ du
+    (stored as the weights are; both or neither).  dx and the weights'
+    gradients are of x's type or fp32."""
+    import torch
+    op, dev = "gated_backward", _device()
+    dt = _type(op, x, "x")
+    M, N, K = _dims(op, x, "x", wg, "wg", b_trans)
+    t16, either = (dt,), (dt, torch.float32)
+    w = (N, K) if b_trans else (K, N)
+    flags = (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
+    pdh, lddh = _mat(op, "dh", dh, t16, M, N, dev)
+    px, ldx = _mat(op, "x", x, t16, M, K, dev)
+    pwg, ldwg = _mat(op, "wg", wg, t16, *w, dev)
+    pwu, ldwu = _mat(op, "wu", wu, t16, *w, dev)
+    pg, ldg = _mat(op, "g", g, t16, M, N, dev)
+    pu, ldu = _mat(op, "u", u, t16, M, N, dev)
+    pdg, lddg = _mat(op, "dg", dg, t16, M, N, dev)
+    pdu, lddu = _mat(op, "du", du, t16, M, N, dev)
+    pdx = pdwg = pdwu = None
+    lddx = lddwg = lddwu = 0
+    if dx is not None:
+        pdx, lddx = _mat(op, "dx", dx, either, M, K, dev)
+        flags |= LINEAR_DA_F32 if dx.dtype is torch.float32 else 0
+    if dwg is not None:
+        pdwg, lddwg = _mat(op, "dwg", dwg, either, *w, dev)
+        flags |= LINEAR_DB_F32 if dwg.dtype is torch.float32 else 0
+    if dwu is not None:
+        pdwu, lddwu = _mat(op, "dwu", dwu, (dwg.dtype,) if dwg is not None else either, *w, dev)
+    check(lib().cudair_gated_backward(ctypes.byref(GatedBackwardArgs(
+        pdh, px, pwg, pwu, pg, pu, pdg, pdu, pdx, pdwg, pdwu, M, N, K, lddh, ldx, ldwg, ldwu, ldg, ldu, lddg,
+        lddu, lddx, lddwg, lddwu, _act(op, act), flags)), _stream(stream)))
 
 
 def gemm_host(a_h, b_h, c_h, a_d, b_d, c_d, rows_per_block=0, stream=None) -> None:

@@ -334,6 +334,112 @@ int cudair_square(float *x, int32_t n, void *stream);
  */
 int cudair_reduce_f32(const float *in, float *out, int32_t n, void *stream);
 
+/* ---- feed-forward layers: fused epilogues, the gated pair, and gradients ---- */
+
+/* The activations.  CUDAIR_ACT_GELU is z P(z) with the normal distribution's
+ * integral P; CUDAIR_ACT_GELU_TANH is z (1 + tanh(sqrt(2/pi) (z + 0.044715
+ * z^3))) / 2; CUDAIR_ACT_SILU is z / (1 + e^-z).  The derivative of RELU at 0
+ * is 0. */
+enum {
+    CUDAIR_ACT_NONE = 0, CUDAIR_ACT_RELU = 1, CUDAIR_ACT_GELU = 2,
+    CUDAIR_ACT_GELU_TANH = 3, CUDAIR_ACT_SILU = 4
+};
+
+/* Flags of the four calls below, beside CUDAIR_GEMM_BF16 (the 16-bit matrices
+ * are bfloat16, else fp16) and CUDAIR_GEMM_B_T (a weight is stored N x K, one
+ * row per output, else K x N). */
+#define CUDAIR_LINEAR_D_F32 0x10u     /* D and the residual, or dY, are fp32 */
+#define CUDAIR_LINEAR_BIAS_16 0x20u   /* the bias is of A's type, else fp32 */
+#define CUDAIR_LINEAR_DA_F32 0x40u    /* dA is fp32 */
+#define CUDAIR_LINEAR_DB_F32 0x80u    /* dB (both weights' gradients) is fp32 */
+
+/*
+ * D = act(Z) + residual with Z = A . B + bias: A (M x K) times a weight B
+ * (K x N, or N x K with CUDAIR_GEMM_B_T), a bias of N values added to every
+ * row, the activation, and a residual (M x N) in one kernel's epilogue.
+ * Stands beside cudair_gemm (the tensor package's MmaF16Bias, tensor.go:31-48,
+ * adds an M x N bias): A and B are both fp16 or both bf16, sums, bias,
+ * activation and residual are fp32, and each output is rounded once.
+ *   bias, residual, z   may be NULL.
+ *   d          M x N of A's type, or fp32 with CUDAIR_LINEAR_D_F32; the
+ *              residual has D's type and may be D itself (same pitch).
+ *   z          M x N of A's type: Z as the backward pass reads it.
+ * Every matrix is row-major with a 16-byte aligned base and a pitch of
+ * whole 16 bytes; pitches are in elements.  No other output may overlap an
+ * input.  M or N of 0 is a no-op; K of 0 gives act(bias) + residual (A and B
+ * are not read).  Needs no workspace, so calls may overlap on several
+ * streams.  Runs on stream, asynchronously, and follows
+ * cudair_set_gemm_pdl.
+ */
+typedef struct cudair_linear_args {
+    const void *a, *b, *bias, *residual;
+    void *d, *z;
+    int64_t M, N, K;
+    int64_t lda, ldb, ldres, ldd, ldz;
+    uint32_t act, flags;
+} cudair_linear_args;
+int cudair_linear(const cudair_linear_args *args, void *stream);
+
+/*
+ * The gradients of cudair_linear.  With dY (M x N, the gradient of D, which is
+ * the residual's gradient as it stands) and Z as the forward pass stored it:
+ *   dZ = dY * act'(Z)        (dz, M x N of A's type)
+ *   dA = dZ . B^T            (M x K; of A's type, or fp32 with _DA_F32)
+ *   dB = A^T . dZ            (stored as B is; of A's type, or fp32 with _DB_F32)
+ *   dbias[n] = sum_m dZ      (N fp32 values, from dZ before it is rounded)
+ * dY is of A's type, or fp32 with CUDAIR_LINEAR_D_F32.  dz is rounded to 16
+ * bits, since it is an operand of the products: it is needed where act is not
+ * CUDAIR_ACT_NONE or dY is fp32, and must be NULL otherwise (dY serves); it
+ * may be dY's or z's own memory (same pitch).  z is needed where act is not
+ * CUDAIR_ACT_NONE.  da, db and dbias may be NULL, and what only they need (b,
+ * a) too.  Outputs are written, not added to.  M of 0 gives dB = 0 and
+ * dbias = 0, N of 0 gives dA = 0.  Layout rules as cudair_linear.
+ */
+typedef struct cudair_linear_backward_args {
+    const void *dy, *a, *b, *z;
+    void *dz, *da, *db;
+    float *dbias;
+    int64_t M, N, K;
+    int64_t lddy, lda, ldb, ldz, lddz, ldda, lddb;
+    uint32_t act, flags;
+} cudair_linear_backward_args;
+int cudair_linear_backward(const cudair_linear_backward_args *args, void *stream);
+
+/*
+ * The gated projection H = act(G) * U with G = X . Wg and U = X . Wu, both
+ * products, the activation and the product in one kernel: X (M x K), Wg and
+ * Wu (K x N, or N x K with CUDAIR_GEMM_B_T), H (M x N), all fp16 or all bf16.
+ * The two weights may be halves of one array (pointers and pitches are
+ * their own).  g and u (M x N, both or neither) receive G and U for the
+ * backward pass.  Other rules as cudair_linear; K of 0 gives H = 0.
+ */
+typedef struct cudair_gated_args {
+    const void *x, *wg, *wu;
+    void *h, *g, *u;
+    int64_t M, N, K;
+    int64_t ldx, ldwg, ldwu, ldh, ldg, ldu;
+    uint32_t act, flags;
+} cudair_gated_args;
+int cudair_gated(const cudair_gated_args *args, void *stream);
+
+/*
+ * The gradients of cudair_gated.  With dH (M x N) and G, U as stored:
+ *   dG = dH * U * act'(G),  dU = dH * act(G)   (dg, du: M x N, 16 bits)
+ *   dX  = dG . Wg^T + dU . Wu^T                (M x K; fp32 with _DA_F32)
+ *   dWg = X^T . dG,  dWu = X^T . dU            (as the weights; fp32 with _DB_F32)
+ * dg and du are needed, and may be g's and u's (or dH's) own memory (same
+ * pitch).  dx may be NULL; dwg and dwu are both given or both NULL.  Other
+ * rules as cudair_linear_backward.
+ */
+typedef struct cudair_gated_backward_args {
+    const void *dh, *x, *wg, *wu, *g, *u;
+    void *dg, *du, *dx, *dwg, *dwu;
+    int64_t M, N, K;
+    int64_t lddh, ldx, ldwg, ldwu, ldg, ldu, lddg, lddu, lddx, lddwg, lddwu;
+    uint32_t act, flags;
+} cudair_gated_backward_args;
+int cudair_gated_backward(const cudair_gated_backward_args *args, void *stream);
+
 /* ---- seeded synthetic operands -------------------------------------------- */
 
 enum { CUDAIR_FILL_F32 = 0, CUDAIR_FILL_F16 = 1 };
