@@ -270,6 +270,9 @@ int product_launch(const Product &p, cudaStream_t stream) {
     unsigned int *status = nullptr;
     CUDAIR_TRY(sm_count_current_device(&sms));
     CUDAIR_TRY(wait_status_current_device(&status));
+    SplitPlan plan;
+    CUDAIR_TRY(split_plan(p, &plan));
+    if (plan.split > 0) return product_split_launch(p, plan, status, stream);
     return product_pair_launch(p, sms, status, stream);
 }
 
@@ -314,6 +317,7 @@ CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     p.bias16 = bias16;
     p.act = static_cast<int>(q->act);
     p.bf16 = q->flags & CUDAIR_GEMM_BF16;
+    p.b_weights = true;
     return product_launch(p, static_cast<cudaStream_t>(stream));
 }
 
@@ -349,6 +353,7 @@ CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
     p.z[1] = out_mat(q->u, q->ldu, false);
     p.act = static_cast<int>(q->act);
     p.bf16 = q->flags & CUDAIR_GEMM_BF16;
+    p.b_weights = true;
     return product_launch(p, static_cast<cudaStream_t>(stream));
 }
 
@@ -423,6 +428,7 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         p.b[0] = operand(q->b, q->ldb, bt);  // the contraction runs over N
         p.d[0] = out_mat(q->da, q->ldda, da_f32);
         p.bf16 = bf16;
+        p.b_weights = true;
         CUDAIR_TRY(product_launch(p, s));
     }
     if (want_db) {
@@ -515,6 +521,7 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         p.b[1] = operand(q->wu, q->ldwu, bt);
         p.d[0] = out_mat(q->dx, q->lddx, dx_f32);
         p.bf16 = bf16;
+        p.b_weights = true;
         CUDAIR_TRY(product_launch(p, s));
     }
     if (want_dw) {

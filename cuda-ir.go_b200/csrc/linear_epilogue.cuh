@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include "../../include/cudair_b200.h"
+#include "linear_internal.h"
 
 namespace cudair {
 namespace ffn {
@@ -19,21 +20,47 @@ namespace ffn {
 //
 //   relu       max(z, 0), a NaN kept
 //   silu       z s(z), s(z) = 1 / (1 + e^-z)
-//   gelu       z P(z), P the normal distribution's integral (normcdff keeps
-//              its relative precision for negative z, where 1 + erf cancels)
+//   gelu       z P(z), P the normal distribution's integral
 //   gelu_tanh  z (1 + tanh(y)) / 2 with y = sqrt(2/pi) (z + 0.044715 z^3),
 //              computed as z s(2y), which is the same and does not cancel
+//
+// An epilogue warp runs 32 columns of these alone on its scheduler, so their
+// length is the epilogue's: with expf, an IEEE division and normcdff a
+// 256-column tile took 18 us (silu, 256 x 1024 outputs; 40 us where the
+// division leaves its fast path) against 2 us without an activation.  So the
+// exponential and the reciprocal are the hardware's (__expf: 2^-22 plus
+// |z| 2^-24 of the value; __fdividef: two units, and 0 for a denominator
+// above 2^126, where the quotient is below 2^-126 anyway).
 
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+// P(z) and E = e^(-z^2 / 2).  The tail is Abramowitz and Stegun's 7.1.26 for
+// erfc(x), x = |z| / sqrt(2): a polynomial in t = 1 / (1 + p x) times e^(-x^2),
+// off by at most 1.5e-7 (so P by 0.75e-7, an fp32 rounding of 1).
+__device__ __forceinline__ void normal_integral(float z, float &P, float &E) {
+    const float x = fabsf(z) * 0.7071067811865476f;
+    E = __expf(-0.5f * z * z);
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float h = fmaf(t, 1.061405429f, -1.453152027f);
+    h = fmaf(t, h, 1.421413741f);
+    h = fmaf(t, h, -0.284496736f);
+    h = fmaf(t, h, 0.254829592f);
+    h *= 0.5f * t * E;
+    P = z < 0.0f ? h : 1.0f - h;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
     if (ACT == CUDAIR_ACT_RELU) return z < 0.0f ? 0.0f : z;
     if (ACT == CUDAIR_ACT_SILU) return z * sigmoid(z);
-    if (ACT == CUDAIR_ACT_GELU) return z * normcdff(z);
+    if (ACT == CUDAIR_ACT_GELU) {
+        float P, E;
+        normal_integral(z, P, E);
+        return z * P;
+    }
     if (ACT == CUDAIR_ACT_GELU_TANH) return z * sigmoid(kGeluC * (z + kGeluB * z * z * z));
     return z;
 }
@@ -49,9 +76,10 @@ __device__ __forceinline__ void act_both(float z, float &value, float &grad) {
         value = z * s;
         grad = s * (1.0f + z * (1.0f - s));
     } else if (ACT == CUDAIR_ACT_GELU) {
-        const float p = normcdff(z);
-        value = z * p;
-        grad = p + z * (0.3989422804014327f * expf(-0.5f * z * z));
+        float P, E;
+        normal_integral(z, P, E);
+        value = z * P;
+        grad = P + z * (0.3989422804014327f * E);
     } else if (ACT == CUDAIR_ACT_GELU_TANH) {
         const float z2 = z * z;
         const float s = sigmoid(kGeluC * (z + kGeluB * z * z2));
@@ -142,6 +170,16 @@ struct Mat {
     int f32;        // 32-bit elements, else 16-bit of the operands' type
     int wide;       // base and pitch are multiples of 32 bytes, else of 16
 };
+
+inline Mat mat_of(const OutMat &m) {
+    const uint64_t bytes = m.f32 ? 4 : 2;
+    Mat r;
+    r.p = m.p;
+    r.ld = static_cast<long long>(m.ld);
+    r.f32 = m.f32;
+    r.wide = ((reinterpret_cast<uintptr_t>(m.p) | (static_cast<uint64_t>(m.ld) * bytes)) & 31u) == 0;
+    return r;
+}
 
 // One row's 32 columns from col (a multiple of 32, below N): whole 32-byte
 // sectors where the matrix allows it, else 16 bytes at a time; the columns of

@@ -40,6 +40,7 @@ struct Product {
     OutMat z[2];                 // plain: Z in z[0]; gated: G and U
     int act = CUDAIR_ACT_NONE;
     bool bf16 = false;
+    bool b_weights = false;      // B is a weight: no kernel of the same call writes it
 };
 
 // Runs the product on the current device: M and N positive, K >= 0.
@@ -47,6 +48,20 @@ int product_launch(const Product &p, cudaStream_t stream);
 
 // The persistent CTA-pair kernel (linear_sm100.cu).
 int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cudaStream_t stream);
+
+// The split kernel (linear_split_sm100.cu): tiles of mt rows x 128 columns,
+// the contraction shared by `split` CTAs with a ring of `stages` each.
+struct SplitPlan {
+    int mt = 0, split = 0, stages = 0;
+};
+int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *status, cudaStream_t stream);
+// How the split kernel should run this product; plan->split is 0 where the
+// pair kernel is the faster one.
+int split_plan(const Product &p, SplitPlan *plan);
+
+// Shared by the two: an operand's tensor map, with boxes of 64 k x box_rows
+// rows where k runs along memory, else of 64 rows x 64 k; 128-byte swizzle.
+int operand_map(CUtensorMap *out, const Operand &o, int64_t rows, int64_t depth, uint32_t box_rows, bool bf16);
 
 }  // namespace ffn
 }  // namespace cudair

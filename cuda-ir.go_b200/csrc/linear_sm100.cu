@@ -356,20 +356,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // ---- host side ---------------------------------------------------------------------
 
-namespace {
-
-Mat mat_of(const OutMat &m) {
-    const uint64_t bytes = m.f32 ? 4 : 2;
-    Mat r;
-    r.p = m.p;
-    r.ld = static_cast<long long>(m.ld);
-    r.f32 = m.f32;
-    r.wide = ((reinterpret_cast<uintptr_t>(m.p) | (static_cast<uint64_t>(m.ld) * bytes)) & 31u) == 0;
-    return r;
-}
-
-// An operand's tensor map: boxes of 64 k x box_rows rows where k runs along
-// memory, else of 64 rows x 64 k; 128-byte swizzle.
 int operand_map(CUtensorMap *out, const Operand &o, int64_t rows, int64_t depth, uint32_t box_rows, bool bf16) {
     const uint64_t dims[2] = {static_cast<uint64_t>(o.mn ? rows : depth),
                               static_cast<uint64_t>(o.mn ? depth : rows)};
@@ -380,6 +366,8 @@ int operand_map(CUtensorMap *out, const Operand &o, int64_t rows, int64_t depth,
                                  CUDAIR_INTERLEAVE_NONE, CUDAIR_SWIZZLE_128B, CUDAIR_L2_PROMOTION_256B,
                                  CUDAIR_OOB_FILL_NONE);
 }
+
+namespace {
 
 std::mutex g_pair_mu;
 int g_pairs[64];  // CTA pairs resident at once, per device (0: not asked yet)

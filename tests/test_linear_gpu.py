@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 # M, N, K: single rows, both sides of 16, 64 and 128 rows, tile edges, odd sizes.
 SHAPES = [(1, 1, 1), (1, 8, 64), (1, 1000, 4096), (2, 131, 70), (7, 515, 1024), (16, 256, 512), (17, 300, 77),
           (33, 1024, 200), (64, 129, 2048), (65, 640, 333), (100, 96, 64), (128, 384, 1000), (129, 257, 65),
-          (200, 72, 4096), (256, 256, 64), (257, 1031, 519), (400, 2050, 136), (1025, 513, 96)]
+          (200, 72, 4096), (256, 256, 64), (257, 1031, 519), (400, 2050, 136), (1025, 513, 96),
+          (257, 5000, 200), (1290, 1031, 1100)]  # enough tiles for the persistent pairs
 FORMS = [  # dtype, rows, act, bias, residual, z, fp32 output, pitch padding, lead
     ("bf16", True, "none", None, True, False, False, 8, 0),
     ("fp16", False, "gelu_tanh", "f32", False, True, False, 0, 8),
@@ -327,6 +328,7 @@ def test_feed_forward_layer(dev, cudair, M, K, F, rows):
     got = [dx.double() + dy.double(), dwg.double(), dwu.double(), dwd.double(), dbd.double()]
     # Up to four roundings to 8 bits (h or g, u; dh; dg, du; the result), each
     # within 2^-9 of a value and independent: 4 x 2^-9 of the norm.
+    want_y = want_y.detach()
     assert float((y.double() - want_y).norm() / want_y.norm()) <= 2 * 2.0 ** -9
     for name, p, q in zip(("dx", "dwg", "dwu", "dwd", "dbd"), got, want):
         rel = float((p - q).norm() / q.norm())
