@@ -23,43 +23,55 @@ namespace ffn {
 constexpr int EW_THREADS = 256;
 constexpr int EW_COLS = 64;              // columns per block: 8 threads of 8 columns
 constexpr int EW_ROWS = EW_THREADS / 8;  // rows per step of a block
-constexpr int EW_BATCH = 4;              // steps whose loads are issued together
 
 struct EwArgs {
     int M, N;
     int chunks;       // blocks per strip of columns
     int rows;         // rows per block
-    int act, bf16, dy_f32;
+    int act;
     const void *dy, *z, *u;  // gated: dH, G, U
     void *dz, *du;           // gated: dG, dU
     long long lddy, ldz, ldu, lddz, lddu;
     float *dbias;
 };
 
-// Eight columns of a row, from a 16-bit or fp32 matrix with 16-byte rows.
-__device__ __forceinline__ void load8(const void *base, long long ld, long long row, int col, int N, bool f32,
-                                      bool bf16, float (&v)[8]) {
-    if (col + 8 <= N) {
-        if (f32) {
-            const float *p = static_cast<const float *>(base) + row * ld + col;
-            uint32_t w[8];
-            ld_v4(p, w);
-            ld_v4(p + 4, w + 4);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
-        } else {
-            uint32_t w[4];
-            ld_v4(static_cast<const uint16_t *>(base) + row * ld + col, w);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) unpack16(w[j], bf16, v[2 * j], v[2 * j + 1]);
-        }
+// Eight columns of a row as they lie in memory: one 16-byte load of 16-bit
+// values, two of fp32.  Not through the read-only path: an output may lie over
+// the matrix.
+struct Raw8 {
+    uint4 lo, hi;
+};
+__device__ __forceinline__ Raw8 load_raw8(const void *base, long long ld, long long row, int col, bool f32) {
+    Raw8 r;
+    if (f32) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(base) + row * ld + col);
+        r.lo = p[0];
+        r.hi = p[1];
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = col + j >= N ? 0.0f
-                   : f32        ? (static_cast<const float *>(base) + row * ld + col)[j]
-                                : from16((static_cast<const uint16_t *>(base) + row * ld + col)[j], bf16);
+        r.lo = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + row * ld + col);
+        r.hi = r.lo;
     }
+    return r;
+}
+__device__ __forceinline__ void convert8(const Raw8 &r, bool f32, bool bf16, float (&v)[8]) {
+    if (f32) {
+        const uint32_t w[8] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w, r.hi.x, r.hi.y, r.hi.z, r.hi.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    } else {
+        const uint32_t w[4] = {r.lo.x, r.lo.y, r.lo.z, r.lo.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpack16(w[j], bf16, v[2 * j], v[2 * j + 1]);
+    }
+}
+// The columns of a last block that ends inside the eight, one by one.
+__device__ __forceinline__ void load8_edge(const void *base, long long ld, long long row, int col, int N, bool f32,
+                                           bool bf16, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        v[j] = col + j >= N ? 0.0f
+               : f32        ? (static_cast<const float *>(base) + row * ld + col)[j]
+                            : from16((static_cast<const uint16_t *>(base) + row * ld + col)[j], bf16);
 }
 __device__ __forceinline__ void store8(void *base, long long ld, long long row, int col, int N, bool bf16,
                                        const float (&v)[8]) {
@@ -76,18 +88,29 @@ __device__ __forceinline__ void store8(void *base, long long ld, long long row, 
     }
 }
 
-// A block takes `rows` rows of one strip of 64 columns, EW_BATCH x 32 rows at
-// a time: all of a batch's loads are issued before its stores, and an element
-// is stored by the thread that loaded it, so the outputs may lie over the
-// inputs.
+// A block takes `rows` rows of one strip of 64 columns, EW_ROWS x BATCH rows
+// at a time.  A batch's loads are all issued before anything waits for one of
+// them (a load and its conversion behind a row check each kept one load in
+// flight per thread: 4096 x 14336 gated took 480 us), and an element is stored
+// by the thread that loaded it, so the outputs may lie over the inputs.
 //
 // SUM (dbias): the blocks of a strip are one cluster of at most eight.  Each
 // adds its rows in fp32 registers, then over its 32 row-threads in shared
 // memory; the cluster's first block reads the others' sums and adds them in
 // rank order.  No atomics and no workspace: the result does not depend on
 // timing, and calls may overlap.
-template <bool GATED, bool SUM>
-__global__ void __launch_bounds__(EW_THREADS) act_grad_kernel(const EwArgs p) {
+// The types are template parameters: chosen at run time, the conversions of both
+// are computed and one kept, and with gelu_tanh the instructions, not the bytes,
+// set the time.
+template <bool GATED, bool F32>
+struct EwCfg {
+    static constexpr int BATCH = GATED || F32 ? 2 : 4;
+    static constexpr int BLOCKS = GATED ? 3 : 4;  // per SM
+};
+
+template <bool GATED, bool SUM, bool bf16, bool f32>
+__global__ void __launch_bounds__(EW_THREADS, (EwCfg<GATED, f32>::BLOCKS)) act_grad_kernel(const EwArgs p) {
+    constexpr int BATCH = EwCfg<GATED, f32>::BATCH;
     __shared__ float part[EW_ROWS][EW_COLS];
     const int strips = (p.N + EW_COLS - 1) / EW_COLS;
     // A strip's blocks next to one another for the cluster; else row by row.
@@ -97,55 +120,81 @@ __global__ void __launch_bounds__(EW_THREADS) act_grad_kernel(const EwArgs p) {
     const int col = strip * EW_COLS + tx * 8;
     const long long first = static_cast<long long>(chunk) * p.rows;
     const long long last = min(first + p.rows, static_cast<long long>(p.M));
-    const bool bf16 = p.bf16 != 0;
+    const bool has_z = GATED || p.act != CUDAIR_ACT_NONE;
     float sum[8] = {};
 
+    auto finish = [&](long long r, float (&dy)[8], const float (&z)[8], const float (&u)[8]) {
+        if (GATED) {
+            float dg[8], du[8];
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float value, grad;
+                    act_both<decltype(tag)::value>(z[j], value, grad);
+                    dg[j] = dy[j] * u[j] * grad;
+                    du[j] = dy[j] * value;
+                }
+            });
+            store8(p.dz, p.lddz, r, col, p.N, bf16, dg);
+            store8(p.du, p.lddu, r, col, p.N, bf16, du);
+        } else {
+            if (has_z)
+                with_act(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float value, grad;
+                        act_both<decltype(tag)::value>(z[j], value, grad);
+                        dy[j] *= grad;
+                    }
+                });
+            if (p.dz) store8(p.dz, p.lddz, r, col, p.N, bf16, dy);
+            if (SUM) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += dy[j];
+            }
+        }
+    };
+
+    if (threadIdx.x == 0) grid_launch_dependents();  // the products may set up
     grid_dependency_wait();
     if (col < p.N) {
-        for (long long r0 = first + ty; r0 < last; r0 += EW_ROWS * EW_BATCH) {
-            float dy[EW_BATCH][8], z[EW_BATCH][8], u[GATED ? EW_BATCH : 1][8];
+        const bool whole = col + 8 <= p.N;
+        long long r0 = first + ty;
+        if (whole)
+            for (; r0 + EW_ROWS * (BATCH - 1) < last; r0 += EW_ROWS * BATCH) {
+                Raw8 dy[BATCH], z[BATCH], u[BATCH];
 #pragma unroll
-            for (int b = 0; b < EW_BATCH; ++b) {
-                const long long r = r0 + b * EW_ROWS;
-                if (r >= last) break;
-                load8(p.dy, p.lddy, r, col, p.N, p.dy_f32, bf16, dy[b]);
-                if (p.z) load8(p.z, p.ldz, r, col, p.N, false, bf16, z[b]);
-                if (GATED) load8(p.u, p.ldu, r, col, p.N, false, bf16, u[GATED ? b : 0]);
-            }
+                for (int b = 0; b < BATCH; ++b) {
+                    const long long r = r0 + b * EW_ROWS;
+                    dy[b] = load_raw8(p.dy, p.lddy, r, col, f32);
+                    if (has_z) z[b] = load_raw8(p.z, p.ldz, r, col, false);
+                    if (GATED) u[b] = load_raw8(p.u, p.ldu, r, col, false);
+                }
 #pragma unroll
-            for (int b = 0; b < EW_BATCH; ++b) {
-                const long long r = r0 + b * EW_ROWS;
-                if (r >= last) break;
-                if (GATED) {
-                    float dg[8], du[8];
-                    with_act(p.act, [&](auto tag) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            float value, grad;
-                            act_both<decltype(tag)::value>(z[b][j], value, grad);
-                            dg[j] = dy[b][j] * u[GATED ? b : 0][j] * grad;
-                            du[j] = dy[b][j] * value;
-                        }
-                    });
-                    store8(p.dz, p.lddz, r, col, p.N, bf16, dg);
-                    store8(p.du, p.lddu, r, col, p.N, bf16, du);
-                } else {
-                    if (p.act != CUDAIR_ACT_NONE)
-                        with_act(p.act, [&](auto tag) {
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                float value, grad;
-                                act_both<decltype(tag)::value>(z[b][j], value, grad);
-                                dy[b][j] *= grad;
-                            }
-                        });
-                    if (p.dz) store8(p.dz, p.lddz, r, col, p.N, bf16, dy[b]);
-                    if (SUM) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) sum[j] += dy[b][j];
-                    }
+                for (int b = 0; b < BATCH; ++b) {
+                    float fy[8], fz[8] = {}, fu[8] = {};
+                    convert8(dy[b], f32, bf16, fy);
+                    if (has_z) convert8(z[b], false, bf16, fz);
+                    if (GATED) convert8(u[b], false, bf16, fu);
+                    finish(r0 + b * EW_ROWS, fy, fz, fu);
                 }
             }
+        for (; r0 < last; r0 += EW_ROWS) {
+            float fy[8], fz[8] = {}, fu[8] = {};
+            if (whole) {
+                const Raw8 dy = load_raw8(p.dy, p.lddy, r0, col, f32);
+                Raw8 z = {}, u = {};
+                if (has_z) z = load_raw8(p.z, p.ldz, r0, col, false);
+                if (GATED) u = load_raw8(p.u, p.ldu, r0, col, false);
+                convert8(dy, f32, bf16, fy);
+                convert8(z, false, bf16, fz);
+                convert8(u, false, bf16, fu);
+            } else {
+                load8_edge(p.dy, p.lddy, r0, col, p.N, f32, bf16, fy);
+                if (has_z) load8_edge(p.z, p.ldz, r0, col, p.N, false, bf16, fz);
+                if (GATED) load8_edge(p.u, p.ldu, r0, col, p.N, false, bf16, fu);
+            }
+            finish(r0, fy, fz, fu);
         }
     }
     if (SUM) {
@@ -176,13 +225,37 @@ __global__ void __launch_bounds__(EW_THREADS) act_grad_kernel(const EwArgs p) {
 
 namespace {
 
-int act_grad_launch(EwArgs &p, bool gated, cudaStream_t stream) {
+template <bool GATED, bool SUM>
+cudaError_t act_grad_start(const cudaLaunchConfig_t &cfg, const EwArgs &p, bool bf16, bool dy_f32) {
+    if (!GATED && dy_f32)
+        return bf16 ? cudaLaunchKernelEx(&cfg, act_grad_kernel<GATED, SUM, true, !GATED>, p)
+                    : cudaLaunchKernelEx(&cfg, act_grad_kernel<GATED, SUM, false, !GATED>, p);
+    return bf16 ? cudaLaunchKernelEx(&cfg, act_grad_kernel<GATED, SUM, true, false>, p)
+                : cudaLaunchKernelEx(&cfg, act_grad_kernel<GATED, SUM, false, false>, p);
+}
+
+int act_grad_launch(EwArgs &p, bool gated, bool bf16, bool dy_f32, int sm_count, cudaStream_t stream) {
     const int64_t strips = (static_cast<int64_t>(p.N) + EW_COLS - 1) / EW_COLS;
     const bool sum = p.dbias != nullptr;
-    const int64_t step = EW_ROWS * EW_BATCH;
+    const int64_t step = EW_ROWS * 4;  // whole batches
     const int64_t steps = (static_cast<int64_t>(p.M) + step - 1) / step;
-    // With a sum, at most eight blocks (a portable cluster) share a strip.
-    const int64_t chunks = sum ? (steps < 1 ? 1 : steps < 8 ? steps : 8) : steps;
+    int64_t chunks = steps;
+    if (sum) {
+        // At most eight blocks (a portable cluster) share a strip; of those the
+        // number whose last wave is fullest (224 strips on 592 places: 5 blocks
+        // make 1.9 waves, 8 make 3.03).
+        const int64_t places = static_cast<int64_t>(sm_count) * EwCfg<false, false>::BLOCKS;
+        chunks = 1;
+        double best = 1e30;
+        for (int64_t c = 1; c <= 8 && c <= steps; ++c) {
+            const double t = static_cast<double>((strips * c + places - 1) / places) *
+                             static_cast<double>((steps + c - 1) / c);
+            if (t <= best) {
+                best = t;
+                chunks = c;
+            }
+        }
+    }
     p.chunks = static_cast<int>(chunks);
     p.rows = static_cast<int>((steps + chunks - 1) / chunks * step);
     if (strips * chunks > INT32_MAX)
@@ -200,9 +273,9 @@ int act_grad_launch(EwArgs &p, bool gated, cudaStream_t stream) {
     cfg.stream = stream;
     cfg.attrs = gemm_pdl_mode() > 0 ? attr : attr + 1;
     cfg.numAttrs = (gemm_pdl_mode() > 0 ? 1 : 0) + (sum ? 1 : 0);
-    const cudaError_t e = gated ? cudaLaunchKernelEx(&cfg, act_grad_kernel<true, false>, p)
-                          : sum ? cudaLaunchKernelEx(&cfg, act_grad_kernel<false, true>, p)
-                                : cudaLaunchKernelEx(&cfg, act_grad_kernel<false, false>, p);
+    const cudaError_t e = gated ? act_grad_start<true, false>(cfg, p, bf16, dy_f32)
+                          : sum ? act_grad_start<false, true>(cfg, p, bf16, dy_f32)
+                                : act_grad_start<false, false>(cfg, p, bf16, dy_f32);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "act_grad_kernel launch");
 }
 
@@ -266,13 +339,13 @@ OutMat out_mat(void *p, int64_t ld, bool f32) {
 }  // namespace
 
 int product_launch(const Product &p, cudaStream_t stream) {
-    int sms = 0;
     unsigned int *status = nullptr;
-    CUDAIR_TRY(sm_count_current_device(&sms));
-    CUDAIR_TRY(wait_status_current_device(&status));
+    CUDAIR_TRY(wait_status_current_device(&status));  // with the device and context checks
     SplitPlan plan;
     CUDAIR_TRY(split_plan(p, &plan));
     if (plan.split > 0) return product_split_launch(p, plan, status, stream);
+    int sms = 0;
+    CUDAIR_TRY(sm_count_current_device(&sms));
     return product_pair_launch(p, sms, status, stream);
 }
 
@@ -406,8 +479,6 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         e.M = static_cast<int>(q->M);
         e.N = static_cast<int>(q->N);
         e.act = static_cast<int>(q->act);
-        e.bf16 = bf16;
-        e.dy_f32 = dy_f32;
         e.dy = q->dy;
         e.z = has_act ? q->z : nullptr;
         e.dz = own_dz ? q->dz : nullptr;
@@ -415,12 +486,13 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         e.ldz = q->ldz;
         e.lddz = q->lddz;
         e.dbias = q->dbias;
-        CUDAIR_TRY(act_grad_launch(e, false, s));
+        CUDAIR_TRY(act_grad_launch(e, false, bf16, dy_f32, sms, s));
     }
     const void *dz = own_dz ? q->dz : q->dy;
     const int64_t lddz = own_dz ? q->lddz : q->lddy;
     if (want_da) {
         Product p;
+        p.chained = elementwise;
         p.M = q->M;
         p.N = q->K;
         p.K = q->N;
@@ -433,6 +505,7 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
     }
     if (want_db) {
         Product p;
+        p.chained = elementwise || want_da;
         p.M = bt ? q->N : q->K;
         p.N = bt ? q->K : q->N;
         p.K = q->M;
@@ -491,12 +564,12 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
     }
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
-    if (q->M > 0 && q->N > 0) {
+    const bool elementwise = q->M > 0 && q->N > 0;
+    if (elementwise) {
         EwArgs e = {};
         e.M = static_cast<int>(q->M);
         e.N = static_cast<int>(q->N);
         e.act = static_cast<int>(q->act);
-        e.bf16 = bf16;
         e.dy = q->dh;
         e.z = q->g;
         e.u = q->u;
@@ -507,11 +580,12 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         e.ldu = q->ldu;
         e.lddz = q->lddg;
         e.lddu = q->lddu;
-        CUDAIR_TRY(act_grad_launch(e, true, s));
+        CUDAIR_TRY(act_grad_launch(e, true, bf16, false, sms, s));
     }
     if (want_dx) {
         Product p;
         p.form = Form::sum;
+        p.chained = elementwise;
         p.M = q->M;
         p.N = q->K;
         p.K = q->N;
@@ -527,6 +601,7 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
     if (want_dw) {
         Product p;
         p.form = Form::pair;
+        p.chained = elementwise || want_dx;
         p.M = bt ? q->N : q->K;
         p.N = bt ? q->K : q->N;
         p.K = q->M;

@@ -41,6 +41,17 @@ struct Product {
     int act = CUDAIR_ACT_NONE;
     bool bf16 = false;
     bool b_weights = false;      // B is a weight: no kernel of the same call writes it
+    // Not the first kernel of its call: it may be launched while the one
+    // before it ends (programmatic dependent launch), whatever the mode of
+    // cudair_set_gemm_pdl.  It waits for that kernel before it reads what the
+    // call computes.
+    bool chained = false;
+
+    bool pdl() const { return chained || gemm_pdl_mode() > 0; }
+    // Whether the weights may be requested before that wait: nothing that is
+    // still running writes them.  A chained kernel's predecessors are the call's own,
+    // unless the call's first kernel overlaps the caller's (mode 1).
+    bool weights_early() const { return b_weights && (gemm_pdl_mode() == 2 || (chained && gemm_pdl_mode() == 0)); }
 };
 
 // Runs the product on the current device: M and N positive, K >= 0.

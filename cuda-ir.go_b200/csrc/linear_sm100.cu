@@ -410,7 +410,7 @@ int resident_pairs(int sm_count, int *pairs) {
 }
 
 template <bool GATED, int NT>
-cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, cudaStream_t stream) {
+cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool pdl, cudaStream_t stream) {
     constexpr int TILE_N = GATED ? NT / 2 : NT;
     const int64_t tiles = static_cast<int64_t>((args.M + static_cast<int64_t>(PM) - 1) / PM) *
                           ((args.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) * args.problems;
@@ -427,7 +427,7 @@ cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, cudaS
     cfg.dynamicSmemBytes = PairCfg<NT>::SMEM;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = gemm_pdl_mode() > 0 ? 2 : 1;
+    cfg.numAttrs = pdl ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NT>, maps, args);
 }
 
@@ -441,11 +441,11 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     alignas(64) Maps maps = {};
     const bool gated = p.form == Form::gated;
     if (p.K > 0) {
-        for (int i = 0; i < 2; ++i) {
-            const int ai = p.form == Form::plain || gated ? 0 : i, bi = p.form == Form::plain ? 0 : i;
-            if ((rc = operand_map(&maps.a[i], p.a[ai], p.M, p.K, 128, p.bf16)) != CUDAIR_OK) return rc;
-            if ((rc = operand_map(&maps.b[i], p.b[bi], p.N, p.K, NT / 2, p.bf16)) != CUDAIR_OK) return rc;
-        }
+        const int as = p.form == Form::plain || gated ? 1 : 2, bs = p.form == Form::plain ? 1 : 2;
+        for (int i = 0; i < as; ++i)
+            if ((rc = operand_map(&maps.a[i], p.a[i], p.M, p.K, 128, p.bf16)) != CUDAIR_OK) return rc;
+        for (int i = 0; i < bs; ++i)
+            if ((rc = operand_map(&maps.b[i], p.b[i], p.N, p.K, NT / 2, p.bf16)) != CUDAIR_OK) return rc;
     }
     PairArgs args = {};
     args.M = static_cast<int>(p.M);
@@ -466,8 +466,8 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     args.bias = p.bias;
     args.bias16 = p.bias16;
     args.status = status;
-    const cudaError_t e = gated ? launch_pair<true, NT>(maps, args, pairs, stream)
-                                : launch_pair<false, NT>(maps, args, pairs, stream);
+    const cudaError_t e = gated ? launch_pair<true, NT>(maps, args, pairs, p.pdl(), stream)
+                                : launch_pair<false, NT>(maps, args, pairs, p.pdl(), stream);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_pair_kernel launch");
 }
 

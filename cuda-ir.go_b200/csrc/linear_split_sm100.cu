@@ -564,13 +564,13 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
     const int w_tiles = gated ? 2 : 1;
     alignas(64) split::Maps maps = {};
     if (p.K > 0) {
-        for (int i = 0; i < 2; ++i) {
-            const int ai = p.form == Form::plain || gated ? 0 : i, bi = p.form == Form::plain ? 0 : i;
-            if ((rc = operand_map(&maps.w[i], p.b[bi], p.N, p.K, NT, p.bf16)) != CUDAIR_OK) return rc;
-            if ((rc = operand_map(&maps.x[i], p.a[ai], p.M, p.K, static_cast<uint32_t>(plan.mt), p.bf16)) !=
+        const int as = p.form == Form::plain || gated ? 1 : 2, bs = p.form == Form::plain ? 1 : 2;
+        for (int i = 0; i < bs; ++i)
+            if ((rc = operand_map(&maps.w[i], p.b[i], p.N, p.K, NT, p.bf16)) != CUDAIR_OK) return rc;
+        for (int i = 0; i < as; ++i)
+            if ((rc = operand_map(&maps.x[i], p.a[i], p.M, p.K, static_cast<uint32_t>(plan.mt), p.bf16)) !=
                 CUDAIR_OK)
                 return rc;
-        }
     }
     split::Args args = {};
     args.M = static_cast<int>(p.M);
@@ -589,7 +589,7 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
     args.tmem_cols = tmem_cols_for(w_tiles, plan.mt);
     args.bf16 = p.bf16;
     args.act = p.act;
-    args.w_early = p.b_weights && gemm_pdl_mode() == 2;
+    args.w_early = p.weights_early();
     for (int i = 0; i < 2; ++i) {
         args.d[i] = mat_of(p.d[i]);
         args.z[i] = mat_of(p.z[i]);
@@ -612,7 +612,7 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = gemm_pdl_mode() > 0 ? 2 : 1;
+    cfg.numAttrs = p.pdl() ? 2 : 1;
     const cudaError_t e = gated ? cudaLaunchKernelEx(&cfg, product_split_kernel<true>, maps, args)
                                 : cudaLaunchKernelEx(&cfg, product_split_kernel<false>, maps, args);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_split_kernel launch");

@@ -139,6 +139,14 @@ def _device():
     return torch.cuda.current_device()
 
 
+def _current_stream(stream, device):
+    """_stream without building a torch Stream object (3 us)."""
+    if stream is None:
+        import torch
+        return torch._C._cuda_getCurrentRawStream(device)
+    return _stream(stream)
+
+
 def _dims(op, x, xname, w, wname, b_trans):
     """(M, N, K) of x (M x K) and a weight (K x N, or N x K with b_trans)."""
     if x.dim() != 2 or w.dim() != 2:
@@ -175,7 +183,7 @@ def linear(a, b, d, bias=None, residual=None, z=None, act="none", b_trans=False,
     if z is not None:
         pz, ldz = _mat(op, "z", z, t16, M, N, dev)
     check(lib().cudair_linear(ctypes.byref(LinearArgs(
-        pa, pb, pbias, pres, pd, pz, M, N, K, lda, ldb, ldres, ldd, ldz, _act(op, act), flags)), _stream(stream)))
+        pa, pb, pbias, pres, pd, pz, M, N, K, lda, ldb, ldres, ldd, ldz, _act(op, act), flags)), _current_stream(stream, dev)))
 
 
 def linear_backward(dy, a, b, z=None, dz=None, da=None, db=None, dbias=None, act="none", b_trans=False,
@@ -217,7 +225,7 @@ def linear_backward(dy, a, b, z=None, dz=None, da=None, db=None, dbias=None, act
         pdbias = _mat(op, "dbias", dbias.view(1, N), (torch.float32,), 1, N, dev)[0]
     check(lib().cudair_linear_backward(ctypes.byref(LinearBackwardArgs(
         pdy, pa, pb, pz, pdz, pda, pdb, pdbias, M, N, K, lddy, lda, ldb, ldz, lddz, ldda, lddb, _act(op, act),
-        flags)), _stream(stream)))
+        flags)), _current_stream(stream, dev)))
 
 
 def gated(x, wg, wu, h, g=None, u=None, act="silu", b_trans=False, stream=None) -> None:
@@ -240,7 +248,7 @@ def gated(x, wg, wu, h, g=None, u=None, act="silu", b_trans=False, stream=None) 
     pu, ldu = (None, 0) if u is None else _mat(op, "u", u, t16, M, N, dev)
     check(lib().cudair_gated(ctypes.byref(GatedArgs(
         px, pwg, pwu, ph, pg, pu, M, N, K, ldx, ldwg, ldwu, ldh, ldg, ldu, _act(op, act), flags)),
-        _stream(stream)))
+        _current_stream(stream, dev)))
 
 
 def gated_backward(dh, x, wg, wu, g, u, dg, du, dx=None, dwg=None, dwu=None, act="silu", b_trans=False,
@@ -277,7 +285,7 @@ def gated_backward(dh, x, wg, wu, g, u, dg, du, dx=None, dwg=None, dwu=None, act
         pdwu, lddwu = _mat(op, "dwu", dwu, (dwg.dtype,) if dwg is not None else either, *w, dev)
     check(lib().cudair_gated_backward(ctypes.byref(GatedBackwardArgs(
         pdh, px, pwg, pwu, pg, pu, pdg, pdu, pdx, pdwg, pdwu, M, N, K, lddh, ldx, ldwg, ldwu, ldg, ldu, lddg,
-        lddu, lddx, lddwg, lddwu, _act(op, act), flags)), _stream(stream)))
+        lddu, lddx, lddwg, lddwu, _act(op, act), flags)), _current_stream(stream, dev)))
 
 
 def gemm_host(a_h, b_h, c_h, a_d, b_d, c_d, rows_per_block=0, stream=None) -> None:
