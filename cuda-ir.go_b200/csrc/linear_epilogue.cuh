@@ -225,49 +225,54 @@ __device__ __forceinline__ void store_row32(const Mat &m, long long row, int col
     }
 }
 
-// Adds one row's 32 columns to v.
-__device__ __forceinline__ void add_row32(const Mat &m, long long row, int col, int N, bool bf16,
-                                          float (&v)[32]) {
+// One row's 32 columns as they lie in memory (16 words of 16-bit values, or
+// 32), so that the loads can be issued long before the values are needed.
+struct Row32 {
+    uint32_t w[32];
+};
+__device__ __forceinline__ void fetch_row32(const Mat &m, long long row, int col, int N, Row32 &r) {
     if (m.f32) {
         const float *p = static_cast<const float *>(m.p) + row * m.ld + col;
         if (col + 32 <= N) {
-            uint32_t w[32];
             if (m.wide) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ld_v8(p + 8 * j, w + 8 * j);
+                for (int j = 0; j < 4; ++j) ld_v8(p + 8 * j, r.w + 8 * j);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ld_v4(p + 4 * j, w + 4 * j);
+                for (int j = 0; j < 8; ++j) ld_v4(p + 4 * j, r.w + 4 * j);
             }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(w[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col + j < N) v[j] += p[j];
+            for (int j = 0; j < 32; ++j) r.w[j] = col + j < N ? __float_as_uint(p[j]) : 0u;
         }
     } else {
         const uint16_t *p = static_cast<const uint16_t *>(m.p) + row * m.ld + col;
         if (col + 32 <= N) {
-            uint32_t w[16];
             if (m.wide) {
-                ld_v8(p, w);
-                ld_v8(p + 16, w + 8);
+                ld_v8(p, r.w);
+                ld_v8(p + 16, r.w + 8);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ld_v4(p + 8 * j, w + 4 * j);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float lo, hi;
-                unpack16(w[j], bf16, lo, hi);
-                v[2 * j] += lo;
-                v[2 * j + 1] += hi;
+                for (int j = 0; j < 4; ++j) ld_v4(p + 8 * j, r.w + 4 * j);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (col + j < N) v[j] += from16(p[j], bf16);
+            for (int j = 0; j < 16; ++j)
+                r.w[j] = (col + 2 * j < N ? p[2 * j] : 0u) | (col + 2 * j + 1 < N ? p[2 * j + 1] : 0u) << 16;
+        }
+    }
+}
+__device__ __forceinline__ void add_row32(const Row32 &r, bool f32, bool bf16, float (&v)[32]) {
+    if (f32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] += __uint_as_float(r.w[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float lo, hi;
+            unpack16(r.w[j], bf16, lo, hi);
+            v[2 * j] += lo;
+            v[2 * j + 1] += hi;
         }
     }
 }

@@ -24,12 +24,16 @@
 // What bounds it: the tensor pipe, for the sizes it is meant for (M > 128;
 // 2 M N K flop against 2 (MK + NK + MN) bytes).  Roles, ring and bounded waits
 // are those of gemm_sm100.cu: warp 0 TMA producer, warp 1 TMEM owner and MMA
-// issuer (even CTA), warps 2-5 epilogue.  Two accumulators of NT columns
-// alternate, so a tile's epilogue runs under the next tile's mainloop.
+// issuer (even CTA), warps 2-9 epilogue (two per lane quarter).  Two
+// accumulators of 256 columns alternate, so a tile's epilogue runs under the
+// next tile's mainloop; or one of 512 columns is handed over in halves.
 //
 // The epilogue writes each thread's row straight from registers, 32 bytes a
 // store (a whole sector): no staging in shared memory, which goes to the ring
-// instead (seven 32 KB stages with NT = 256, nine 24 KB stages with NT = 128).
+// instead (seven 32 KB stages, or four of 48 KB).  The residual's columns are
+// requested ahead of their use, the first before the accumulator is waited for
+// (8192^3 in wide tiles with bias, relu and residual: 947 us with four warps
+// and loads where they are used, 905 us).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -44,23 +48,30 @@ namespace cudair {
 namespace ffn {
 
 constexpr int BK = 64;
-constexpr int THREADS = 192;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int PM = 256;  // rows per pair tile, 128 per CTA
 constexpr uint32_t A_STAGE = 128 * BK * 2;
 constexpr uint32_t BAR_BYTES = 256;
 constexpr int GROUP_M = 8;  // row-blocks visited together (A and B panels shared in L2)
 
-template <int NT>
+// A tile takes NB accumulator blocks of BN columns (the MMA's N).  NB = 1: two
+// accumulators that alternate.  NB = 2: one of 512 columns that fills TMEM, for a
+// quarter fewer operand bytes per flop.  (BN = 128 tiles for outputs of few
+// tiles gain nothing: a 256 x 128 MMA takes as long as a 256 x 256 one, 512 x
+// 4096 x 4096 26.1 against 26.4 us.)
+constexpr int BN = 256;
+template <int NB>
 struct PairCfg {
-    static constexpr int HALF = NT / 2;  // B columns per CTA
-    static constexpr uint32_t B_STAGE = HALF * BK * 2;
+    static constexpr uint32_t B_BLOCK = BN / 2 * BK * 2;  // this CTA's half of a block
+    static constexpr uint32_t B_STAGE = NB * B_BLOCK;
     static constexpr uint32_t STAGE = A_STAGE + B_STAGE;
     static constexpr int STAGES = static_cast<int>((227 * 1024 - 1024 - BAR_BYTES) / STAGE);
-    static constexpr uint32_t TMEM_COLS = 2 * NT;
     static constexpr size_t SMEM = 1024 + STAGES * STAGE + BAR_BYTES;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
     static_assert(2 * STAGES * 8 + 5 * 8 + 8 <= BAR_BYTES, "barrier area");
 };
+constexpr uint32_t TMEM_COLS = 512;
 
 struct Maps {
     CUtensorMap a[2], b[2];
@@ -111,12 +122,70 @@ __device__ __forceinline__ void load_acc(bool any, uint32_t taddr, float (&v)[32
     }
 }
 
-template <bool GATED, int NT>
+// Columns of D that one epilogue warp takes of an accumulator block: two warps
+// share the block's 32 rows of a TMEM lane quarter.
+template <bool GATED>
+constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
+
+// One warp's 32 rows (one per lane) and kWarpCols columns from n0 on; t_row is
+// where they start in TMEM.  `next` holds the residual's first 32 columns,
+// requested before the accumulator was waited for; each further 32 are
+// requested while the ones before them are worked on.
+template <bool GATED>
+__device__ __forceinline__ void epilogue_block(const PairArgs &p, uint32_t t_row, int prob, int row, int n0, bool live,
+                                               bool any, Row32 &next) {
+    const bool bf16 = p.bf16 != 0;
+#pragma unroll 1
+    for (int c = 0; c < kWarpCols<GATED>; c += 32) {
+        const int col = n0 + c;
+        if (col >= p.N) break;
+        float v[32];
+        load_acc(any, t_row + c, v);
+        if (GATED) {
+            float u[32];
+            load_acc(any, t_row + BN / 2 + c, u);
+            if (p.z[0].p && live) {
+                store_row32(p.z[0], row, col, p.N, bf16, v);
+                store_row32(p.z[1], row, col, p.N, bf16, u);
+            }
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]) * u[j];
+            });
+        } else {
+            if (p.bias) {
+                // Lane l reads column l's bias; a shuffle hands it on.
+                float b = 0.0f;
+                const int bc = col + static_cast<int>(lane_id());
+                if (bc < p.N)
+                    b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
+                                 : static_cast<const float *>(p.bias)[bc];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
+            }
+            if (p.z[0].p && live) store_row32(p.z[0], row, col, p.N, bf16, v);
+            if (p.act != CUDAIR_ACT_NONE)
+                with_act(p.act, [&](auto tag) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
+                });
+            if (p.residual.p && live) {
+                add_row32(next, p.residual.f32, bf16, v);
+                if (c + 32 < kWarpCols<GATED> && col + 32 < p.N)
+                    fetch_row32(p.residual, row, col + 32, p.N, next);
+            }
+        }
+        if (live) store_row32(p.d[prob], row, col, p.N, bf16, v);
+    }
+}
+
+template <bool GATED, int NB>
 __global__ void __launch_bounds__(THREADS, 1)
     product_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ PairArgs p) {
-    using Cfg = PairCfg<NT>;
+    using Cfg = PairCfg<NB>;
     constexpr int STAGES = Cfg::STAGES;
-    constexpr int TILE_N = GATED ? Cfg::HALF : NT;  // columns of D per tile
+    constexpr int BLOCK_N = GATED ? BN / 2 : BN;  // columns of D per accumulator block
+    constexpr int TILE_N = NB * BLOCK_N;        // ... and per tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t *smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);  // same offset in both CTAs
@@ -150,14 +219,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 8);  // the epilogue warps of both CTAs
+            mbar_init(&acc_empty[b], 2 * EPI_WARPS);  // those of both CTAs
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 1) {
-        tmem_alloc_pair(tmem_slot, Cfg::TMEM_COLS);
+        tmem_alloc_pair(tmem_slot, TMEM_COLS);
         tmem_relinquish_pair();
     }
     tc_fence_before_sync();
@@ -182,7 +251,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // Rows and columns beyond the matrices arrive as zeros (the
                 // maps clip), so every stage carries the same bytes.
                 const int m_mine = m_blk * PM + 128 * static_cast<int>(rank);
-                const int n_mine = n_blk * TILE_N + (GATED ? 0 : Cfg::HALF * static_cast<int>(rank));
+                // A block takes the first half of its columns of B from the even
+                // CTA, the others from the odd one: of one weight, or (gated)
+                // of the two.
+                const int n_mine = n_blk * TILE_N + (GATED ? 0 : BN / 2 * static_cast<int>(rank));
                 for (int kb = 0; kb < num_kb; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteProducerEmpty)) {
                         give_up();
@@ -203,12 +275,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                     } else {
                         tma_load_2d_pair(da, ma, full_even, k0, m_mine, policy);
                     }
-                    if (p.b_mn) {
 #pragma unroll
-                        for (int j = 0; j < Cfg::HALF / 64; ++j)
-                            tma_load_2d_pair(db + j * 64 * BK * 2, mb, full_even, n_mine + 64 * j, k0, policy);
-                    } else {
-                        tma_load_2d_pair(db, mb, full_even, k0, n_mine, policy);
+                    for (int h = 0; h < NB; ++h) {
+                        uint8_t *dh = db + h * Cfg::B_BLOCK;
+                        const int n = n_mine + h * BLOCK_N;
+                        if (p.b_mn) {
+#pragma unroll
+                            for (int j = 0; j < BN / 2; j += 64)
+                                tma_load_2d_pair(dh + j * BK * 2, mb, full_even, n + j, k0, policy);
+                        } else {
+                            tma_load_2d_pair(dh, mb, full_even, k0, n, policy);
+                        }
                     }
                     if (++stage == STAGES) {
                         stage = 0;
@@ -232,36 +309,85 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint32_t b_step = p.b_mn ? 2048u : 32u, b_lbo = p.b_mn ? 64u * BK * 2 : 16u;
             uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
             bool ok = true, issued_any = false;
-            for (int t = cluster; t < num_tiles && ok; t += num_clusters) {
-                if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u, abort_flag, p.status, kSiteMmaAccEmpty)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after_sync();
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, kSiteMmaFull)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    const uint32_t a_base = smem_u32(sA + stage * A_STAGE);
-                    const uint32_t b_base = smem_u32(sB + stage * Cfg::B_STAGE);
+            // The MMAs of the k-block in stage st into blocks [lo, hi) of the
+            // accumulator; `first` overwrites it.
+            auto issue = [&](uint32_t st, bool first, int lo, int hi) {
+                const uint32_t a_base = smem_u32(sA + st * A_STAGE);
+                const uint32_t b_base = smem_u32(sB + st * Cfg::B_STAGE);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; ++kk)
-                        umma_f16_ss_pair(tmem_base + acc * NT, smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024),
-                                         smem_desc_sw128(b_base + kk * b_step, b_lbo, 1024), p.idesc,
-                                         (kb | kk) != 0 ? 1u : 0u);
-                    issued_any = true;
-                    umma_commit_pair_multicast(&empty[stage], 0x3);
-                    if (++stage == STAGES) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                for (int kk = 0; kk < BK / 16; ++kk) {
+                    const uint64_t a_desc = smem_desc_sw128(a_base + kk * a_step, a_lbo, 1024);
+                    for (int h = lo; h < hi; ++h)
+                        umma_f16_ss_pair(tmem_base + (acc + h) * BN, a_desc,
+                                         smem_desc_sw128(b_base + h * Cfg::B_BLOCK + kk * b_step, b_lbo, 1024),
+                                         p.idesc, first && kk == 0 ? 0u : 1u);
                 }
-                if (!ok) break;
-                umma_commit_pair_multicast(&acc_full[acc], 0x3);
-                acc ^= 1u;
-                if (acc == 0) acc_phase ^= 1u;
+                issued_any = true;
+            };
+            auto wait_full = [&]() {
+                if (!mbar_wait(&full[stage], phase, abort_flag, p.status, kSiteMmaFull)) return false;
+                tc_fence_after_sync();
+                return true;
+            };
+            auto wait_acc = [&](uint32_t b) {
+                if (!mbar_wait(&acc_empty[b], acc_phase ^ 1u, abort_flag, p.status, kSiteMmaAccEmpty)) return false;
+                tc_fence_after_sync();
+                return true;
+            };
+            auto advance = [&]() {
+                if (++stage == STAGES) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            // k-blocks [lo, hi), all blocks, releasing each stage.
+            auto plain = [&](int lo, int hi) {
+                for (int kb = lo; kb < hi; ++kb) {
+                    if (!wait_full()) return false;
+                    issue(stage, kb == 0, 0, NB);
+                    umma_commit_pair_multicast(&empty[stage], 0x3);
+                    advance();
+                }
+                return true;
+            };
+            // NB = 2: one accumulator cannot be drained under the next tile's
+            // mainloop, so its two blocks are handed over separately.  In a
+            // tile's first and last ring-full of k-blocks, block 0 is
+            // multiplied for all of them before block 1: block 0's epilogue
+            // starts while block 1's last MMAs run, and the next tile starts
+            // on block 0 while block 1 is being drained.
+            auto window = [&](int lo, int hi, bool first, bool last) {
+                const uint32_t st0 = stage;
+                if (first && !wait_acc(0)) return false;
+                for (int kb = lo; kb < hi; ++kb) {
+                    if (!wait_full()) return false;
+                    issue(stage, kb == 0, 0, 1);
+                    advance();
+                }
+                if (last) umma_commit_pair_multicast(&acc_full[0], 0x3);
+                if (first && !wait_acc(1)) return false;
+                uint32_t st = st0;
+                for (int kb = lo; kb < hi; ++kb) {
+                    issue(st, kb == 0, 1, 2);
+                    umma_commit_pair_multicast(&empty[st], 0x3);
+                    if (++st == STAGES) st = 0;
+                }
+                if (last) umma_commit_pair_multicast(&acc_full[1], 0x3);
+                return true;
+            };
+            for (int t = cluster; t < num_tiles && ok; t += num_clusters) {
+                if (NB == 2) {
+                    const int head = min(STAGES, num_kb), tail = max(head, num_kb - STAGES);
+                    ok = window(0, head, true, head == num_kb) && plain(head, tail) &&
+                         (tail == num_kb || window(tail, num_kb, false, true));
+                    acc_phase ^= 1u;
+                } else {
+                    ok = wait_acc(acc) && plain(0, num_kb);
+                    if (!ok) break;
+                    umma_commit_pair_multicast(&acc_full[acc], 0x3);
+                    acc ^= 1u;
+                    if (acc == 0) acc_phase ^= 1u;
+                }
             }
             if (!ok) {
                 give_up();
@@ -273,10 +399,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         __syncwarp();
     } else {
-        // ---------------- epilogue (warps 2..5, both CTAs) ----------------
+        // ---------------- epilogue (warps 2..9, both CTAs) ----------------
         grid_dependency_wait();  // the outputs may be the preceding kernel's inputs
         const uint32_t q = warp & 3u;  // the TMEM lane quarter this warp may read
-        const bool bf16 = p.bf16 != 0;
+        const int side = static_cast<int>(warp - 2u) / 4;  // which of the quarter's warps
         uint32_t acc = 0, acc_phase = 0;
         for (int t = cluster; t < num_tiles; t += num_clusters) {
             const int prob = t / per_problem;
@@ -286,58 +412,31 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int row = row0 + static_cast<int>(lane);
             const int n0 = n_blk * TILE_N;
             const bool live = row < p.M;
-            if (num_kb > 0) {
-                if (!mbar_wait(&acc_full[acc], acc_phase, abort_flag, p.status, kSiteEpilogueAccFull)) {
-                    give_up();
-                    break;
-                }
-                tc_fence_after_sync();
-            }
-            const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * NT;
-            if (row0 < p.M) {  // the whole warp: TMEM loads are warp-wide
+            bool aborted = false;
 #pragma unroll 1
-                for (int c = 0; c < TILE_N; c += 32) {
-                    const int col = n0 + c;
-                    if (col >= p.N) break;
-                    float v[32];
-                    load_acc(num_kb > 0, t_row + c, v);
-                    if (GATED) {
-                        float u[32];
-                        load_acc(num_kb > 0, t_row + Cfg::HALF + c, u);
-                        if (p.z[0].p && live) {
-                            store_row32(p.z[0], row, col, p.N, bf16, v);
-                            store_row32(p.z[1], row, col, p.N, bf16, u);
-                        }
-                        with_act(p.act, [&](auto tag) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]) * u[j];
-                        });
-                    } else {
-                        if (p.bias) {
-                            // Lane l reads column l's bias; a shuffle hands it on.
-                            float b = 0.0f;
-                            const int bc = col + static_cast<int>(lane);
-                            if (bc < p.N)
-                                b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
-                                             : static_cast<const float *>(p.bias)[bc];
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
-                        }
-                        if (p.z[0].p && live) store_row32(p.z[0], row, col, p.N, bf16, v);
-                        if (p.act != CUDAIR_ACT_NONE)
-                            with_act(p.act, [&](auto tag) {
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
-                            });
-                        if (p.residual.p && live) add_row32(p.residual, row, col, p.N, bf16, v);
+            for (int h = 0; h < NB; ++h) {
+                const uint32_t bar = acc + h;  // NB = 2: block h's own barriers
+                const int col0 = n0 + h * BLOCK_N + side * kWarpCols<GATED>;
+                Row32 res;
+                if (!GATED && p.residual.p && live && col0 < p.N) fetch_row32(p.residual, row, col0, p.N, res);
+                if (num_kb > 0) {
+                    if (!mbar_wait(&acc_full[bar], acc_phase, abort_flag, p.status, kSiteEpilogueAccFull)) {
+                        give_up();
+                        aborted = true;
+                        break;
                     }
-                    if (live) store_row32(p.d[prob], row, col, p.N, bf16, v);
+                    __syncwarp();
+                    tc_fence_after_sync();
                 }
+                const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + side * kWarpCols<GATED>;
+                if (row0 < p.M)  // the whole warp: TMEM loads are warp-wide
+                    epilogue_block<GATED>(p, t_row, prob, row, col0, live, num_kb > 0, res);
+                tc_fence_before_sync();
+                __syncwarp();
+                if (num_kb > 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[bar]), 0));
             }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (num_kb > 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[acc]), 0));
-            acc ^= 1u;
+            if (aborted) break;
+            if (NB == 1) acc ^= 1u;
             if (acc == 0) acc_phase ^= 1u;
         }
         __syncwarp();
@@ -350,7 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     cluster_sync();
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc_pair(tmem_base, Cfg::TMEM_COLS);
+        tmem_dealloc_pair(tmem_base, TMEM_COLS);
     }
 }
 
@@ -372,11 +471,11 @@ namespace {
 std::mutex g_pair_mu;
 int g_pairs[64];  // CTA pairs resident at once, per device (0: not asked yet)
 
-template <bool GATED, int NT>
+template <bool GATED, int NB>
 cudaError_t prepare_kernel(int sm_count, int *clusters) {
-    cudaError_t e = cudaFuncSetAttribute(product_pair_kernel<GATED, NT>,
+    cudaError_t e = cudaFuncSetAttribute(product_pair_kernel<GATED, NB>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(PairCfg<NT>::SMEM));
+                                         static_cast<int>(PairCfg<NB>::SMEM));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
@@ -386,10 +485,10 @@ cudaError_t prepare_kernel(int sm_count, int *clusters) {
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (sm_count / 2)), 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = PairCfg<NT>::SMEM;
+    cfg.dynamicSmemBytes = PairCfg<NB>::SMEM;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaOccupancyMaxActiveClusters(clusters, product_pair_kernel<GATED, NT>, &cfg);
+    return cudaOccupancyMaxActiveClusters(clusters, product_pair_kernel<GATED, NB>, &cfg);
 }
 
 int resident_pairs(int sm_count, int *pairs) {
@@ -399,8 +498,9 @@ int resident_pairs(int sm_count, int *pairs) {
     std::lock_guard<std::mutex> lk(g_pair_mu);  // dev is in 0..63: the device check passed
     if (g_pairs[dev] == 0) {
         int n = 0;
-        if ((e = prepare_kernel<false, 256>(sm_count, &n)) != cudaSuccess ||
-            (e = prepare_kernel<true, 256>(sm_count, &n)) != cudaSuccess)
+        if ((e = prepare_kernel<false, 1>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<false, 2>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<true, 1>(sm_count, &n)) != cudaSuccess)
             return cuda_error(e, "product_pair_kernel set-up");
         if (n < 1) return set_error(CUDAIR_ERR_CUDA, "cudair: no CTA pair of the linear kernels fits this device");
         g_pairs[dev] = n;
@@ -409,9 +509,25 @@ int resident_pairs(int sm_count, int *pairs) {
     return CUDAIR_OK;
 }
 
-template <bool GATED, int NT>
+// Whether 256 x 512 tiles (NB = 2) beat 256 x 256 ones: waves of tiles times a
+// tile's time, in microseconds fitted on B200 (8192^3: 14 waves of 256 x 256
+// tiles 898 us against 7 of the wide ones 855 us, back to back; 2048 x 14336 x
+// 4096: 7 waves 165 us against 4 waves 198 us).  With A's rows along memory (weight
+// gradients) the narrow tile costs more: dWg, dWu of 14336 x 4096 over 4096
+// rows, 25 waves 777 us against 13 waves 736 us.  gated keeps 256 x 256: its
+// epilogue is long enough to want two accumulators (4096 x 14336 x 4096 719
+// against 726 us, 744 against 781 us with G and U stored).
+bool wide_tiles(const Product &p, int pairs) {
+    const int64_t mt = (p.M + PM - 1) / PM * (p.form == Form::pair ? 2 : 1);
+    const double k = static_cast<double>(p.K) * (p.form == Form::sum ? 2 : 1);
+    const double w1 = static_cast<double>((mt * ((p.N + 255) / 256) + pairs - 1) / pairs);
+    const double w2 = static_cast<double>((mt * ((p.N + 511) / 512) + pairs - 1) / pairs);
+    return w2 * (0.0112 * k + 4.5) < w1 * ((p.a[0].mn ? 0.0066 : 0.0059) * k + 0.2);
+}
+
+template <bool GATED, int NB>
 cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool pdl, cudaStream_t stream) {
-    constexpr int TILE_N = GATED ? NT / 2 : NT;
+    constexpr int TILE_N = NB * (GATED ? BN / 2 : BN);
     const int64_t tiles = static_cast<int64_t>((args.M + static_cast<int64_t>(PM) - 1) / PM) *
                           ((args.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) * args.problems;
     cudaLaunchConfig_t cfg = {};
@@ -424,11 +540,11 @@ cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = PairCfg<NT>::SMEM;
+    cfg.dynamicSmemBytes = PairCfg<NB>::SMEM;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NT>, maps, args);
+    return cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NB>, maps, args);
 }
 
 }  // namespace
@@ -437,7 +553,6 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     int pairs = 0;
     int rc = resident_pairs(sm_count, &pairs);
     if (rc != CUDAIR_OK) return rc;
-    constexpr int NT = 256;
     alignas(64) Maps maps = {};
     const bool gated = p.form == Form::gated;
     if (p.K > 0) {
@@ -445,7 +560,7 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
         for (int i = 0; i < as; ++i)
             if ((rc = operand_map(&maps.a[i], p.a[i], p.M, p.K, 128, p.bf16)) != CUDAIR_OK) return rc;
         for (int i = 0; i < bs; ++i)
-            if ((rc = operand_map(&maps.b[i], p.b[i], p.N, p.K, NT / 2, p.bf16)) != CUDAIR_OK) return rc;
+            if ((rc = operand_map(&maps.b[i], p.b[i], p.N, p.K, BN / 2, p.bf16)) != CUDAIR_OK) return rc;
     }
     PairArgs args = {};
     args.M = static_cast<int>(p.M);
@@ -455,7 +570,7 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     args.problems = p.form == Form::pair ? 2 : 1;
     args.a_mn = p.a[0].mn;
     args.b_mn = p.b[0].mn;
-    args.idesc = idesc_f16_f32(PM, NT, p.a[0].mn, p.b[0].mn, p.bf16);
+    args.idesc = idesc_f16_f32(PM, BN, p.a[0].mn, p.b[0].mn, p.bf16);
     args.bf16 = p.bf16;
     args.act = p.act;
     for (int i = 0; i < 2; ++i) {
@@ -466,8 +581,10 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     args.bias = p.bias;
     args.bias16 = p.bias16;
     args.status = status;
-    const cudaError_t e = gated ? launch_pair<true, NT>(maps, args, pairs, p.pdl(), stream)
-                                : launch_pair<false, NT>(maps, args, pairs, p.pdl(), stream);
+    const bool pdl = p.pdl();
+    const cudaError_t e = gated                 ? launch_pair<true, 1>(maps, args, pairs, pdl, stream)
+                          : wide_tiles(p, pairs) ? launch_pair<false, 2>(maps, args, pairs, pdl, stream)
+                                                : launch_pair<false, 1>(maps, args, pairs, pdl, stream);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_pair_kernel launch");
 }
 

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 SHAPES = [(1, 1, 1), (1, 8, 64), (1, 1000, 4096), (2, 131, 70), (7, 515, 1024), (16, 256, 512), (17, 300, 77),
           (33, 1024, 200), (64, 129, 2048), (65, 640, 333), (100, 96, 64), (128, 384, 1000), (129, 257, 65),
           (200, 72, 4096), (256, 256, 64), (257, 1031, 519), (400, 2050, 136), (1025, 513, 96),
-          (257, 5000, 200), (1290, 1031, 1100)]  # enough tiles for the persistent pairs
+          (257, 5000, 200), (1290, 1031, 1100), (600, 2050, 5000)]  # enough tiles for the persistent pairs
 FORMS = [  # dtype, rows, act, bias, residual, z, fp32 output, pitch padding, lead
     ("bf16", True, "none", None, True, False, False, 8, 0),
     ("fp16", False, "gelu_tanh", "f32", False, True, False, 0, 8),
