@@ -1,10 +1,10 @@
 // linear_sm100.cu - the products of the feed-forward operators (cudair_linear,
 // cudair_gated and their gradients) on persistent CTA pairs.
 //
-//   plain   D = act(A.B + bias) + residual, Z = A.B + bias kept if asked
-//   gated   H = act(A.Wg) * (A.Wu), both products kept if asked
-//   sum     dX = dG.Wg^T + dU.Wu^T: one accumulator over both contractions
-//   pair    dWg = X^T.dG and dWu = X^T.dU: one grid over both problems
+//   linear    D = act(A.B + bias) + residual, Z = A.B + bias kept if asked
+//   gated     H = act(A.Wg) * (A.Wu), both products kept if asked
+//   gradients dA = dZ.B^T and dB = A^T.dZ; dX = dG.Wg^T + dU.Wu^T, dWg = X^T.dG
+//             and dWu = X^T.dU: up to three jobs in one launch
 //
 // Mathematics.  Every one of these is a sum over k of 16-bit products held in
 // fp32 (TMEM), then a function of one or two accumulators element by element.
@@ -15,8 +15,10 @@
 //     The even CTA loads Wg's columns and the odd CTA Wu's, so one accumulator
 //     row holds G in its first half and U in its second: the epilogue thread
 //     that owns the row has both without an exchange, and X is read once.
-//   sum: k-blocks past the first contraction's end come from the second pair
-//     of maps and go into the same accumulator; dX is written once.
+//   dX: k-blocks past the first contraction's end come from the second pair of
+//     maps and go into the same accumulator; dX is written once.
+//   several jobs: their tiles are dealt out together, long ones first, so that
+//     no job ends on a wave of its own that leaves SMs idle.
 //   transposed operands (dA = dZ.B^T, dB = A^T.dZ, weights stored N x K) are
 //     read as they lie in memory: the shared-memory descriptors say whether k
 //     or the rows run along a tile's 128-byte swizzle rows.
@@ -38,6 +40,7 @@
 #include <cuda_runtime.h>
 
 #include <mutex>
+#include <utility>
 
 #include "cudair_internal.h"
 #include "linear_epilogue.cuh"
@@ -74,22 +77,60 @@ struct PairCfg {
 constexpr uint32_t TMEM_COLS = 512;
 
 struct Maps {
-    CUtensorMap a[2], b[2];
+    CUtensorMap a[kMaxJobs][2], b[kMaxJobs][2];
 };
 
-struct PairArgs {
-    int M, N;
-    int num_kb;   // k-blocks of one contraction
-    int parts;    // contractions per accumulator (sum: 2)
-    int problems; // independent problems (pair: 2)
+struct JobArgs {
+    int M, N, num_m, num_n;
+    int num_kb, parts;  // k-blocks of one contraction; contractions per accumulator
     int a_mn, b_mn;
     uint32_t idesc;
+    Mat d;
+};
+
+// The tiles of all jobs are numbered through, job after job.  Job 0 has the
+// longest ones: pair c takes its tiles c, c + C, ... (C pairs), so the first
+// pairs get one more than the others.  Of the rest every pair takes `rounds`, a
+// round that is not full from the last pair down, and the pairs with one long
+// tile less share what remains: all end at about the same time.
+struct PairArgs {
+    JobArgs job[kMaxJobs];
+    int first[kMaxJobs + 1];  // a job's first tile; the end
+    int rounds;
     int bf16, act;
-    Mat d[2], z[2], residual;
+    Mat z[2], residual;
     const void *bias;
     int bias16;
     unsigned int *status;
 };
+
+// The i-th tile of pair c of C, -1 after its last.
+__device__ __forceinline__ int tile_of(const PairArgs &p, int i, int c, int C) {
+    const int n0 = p.first[1], end = p.first[kMaxJobs];
+    const int more = n0 % C;  // pairs with one more tile of job 0
+    const int own = n0 / C + (c < more ? 1 : 0);
+    if (i < own) return i * C + c;
+    const int j = i - own;
+    int t = end;
+    if (j < p.rounds)
+        t = n0 + j * C + C - 1 - c;
+    else if (c >= more)
+        t = n0 + p.rounds * C + (j - p.rounds) * (C - more) + C - 1 - c;
+    return t < end ? t : -1;
+}
+template <int V>
+struct Index {
+    static constexpr int value = V;
+};
+__device__ __forceinline__ int job_of(const PairArgs &p, int t) {
+    return (t >= p.first[1] ? 1 : 0) + (t >= p.first[2] ? 1 : 0);
+}
+// A copy in registers, from fixed places in the arguments: an indexed place is
+// read through memory, again at every use between the kernel's asm statements
+// (gated 4096 x 14336 x 4096: 750 against 641 us).
+__device__ __forceinline__ JobArgs job_at(const PairArgs &p, int j) {
+    return j == 0 ? p.job[0] : j == 1 ? p.job[1] : p.job[2];
+}
 
 __device__ __forceinline__ void drain_wait(uint64_t *bar, uint32_t parity, unsigned int *status) {
     int never = 0;
@@ -132,21 +173,21 @@ constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
 // requested before the accumulator was waited for; each further 32 are
 // requested while the ones before them are worked on.
 template <bool GATED>
-__device__ __forceinline__ void epilogue_block(const PairArgs &p, uint32_t t_row, int prob, int row, int n0, bool live,
+__device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row, int n0, bool live,
                                                bool any, Row32 &next) {
     const bool bf16 = p.bf16 != 0;
 #pragma unroll 1
     for (int c = 0; c < kWarpCols<GATED>; c += 32) {
         const int col = n0 + c;
-        if (col >= p.N) break;
+        if (col >= job.N) break;
         float v[32];
         load_acc(any, t_row + c, v);
         if (GATED) {
             float u[32];
             load_acc(any, t_row + BN / 2 + c, u);
             if (p.z[0].p && live) {
-                store_row32(p.z[0], row, col, p.N, bf16, v);
-                store_row32(p.z[1], row, col, p.N, bf16, u);
+                store_row32(p.z[0], row, col, job.N, bf16, v);
+                store_row32(p.z[1], row, col, job.N, bf16, u);
             }
             with_act(p.act, [&](auto tag) {
 #pragma unroll
@@ -157,13 +198,13 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, uint32_t t_row
                 // Lane l reads column l's bias; a shuffle hands it on.
                 float b = 0.0f;
                 const int bc = col + static_cast<int>(lane_id());
-                if (bc < p.N)
+                if (bc < job.N)
                     b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
                                  : static_cast<const float *>(p.bias)[bc];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
             }
-            if (p.z[0].p && live) store_row32(p.z[0], row, col, p.N, bf16, v);
+            if (p.z[0].p && live) store_row32(p.z[0], row, col, job.N, bf16, v);
             if (p.act != CUDAIR_ACT_NONE)
                 with_act(p.act, [&](auto tag) {
 #pragma unroll
@@ -171,11 +212,11 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, uint32_t t_row
                 });
             if (p.residual.p && live) {
                 add_row32(next, p.residual.f32, bf16, v);
-                if (c + 32 < kWarpCols<GATED> && col + 32 < p.N)
-                    fetch_row32(p.residual, row, col + 32, p.N, next);
+                if (c + 32 < kWarpCols<GATED> && col + 32 < job.N)
+                    fetch_row32(p.residual, row, col + 32, job.N, next);
             }
         }
-        if (live) store_row32(p.d[prob], row, col, p.N, bf16, v);
+        if (live) store_row32(job.d, row, col, job.N, bf16, v);
     }
 }
 
@@ -205,11 +246,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t rank = cluster_ctarank();  // 0 = even CTA (issues the MMAs)
     const int cluster = static_cast<int>(blockIdx.x >> 1);
     const int num_clusters = static_cast<int>(gridDim.x >> 1);
-    const int num_m = (p.M + PM - 1) / PM;
-    const int num_n = (p.N + TILE_N - 1) / TILE_N;
-    const int per_problem = num_m * num_n;
-    const int num_tiles = per_problem * p.problems;
-    const int num_kb = p.num_kb * p.parts;
     const uint32_t peer_abort = mapa_shared(smem_u32(const_cast<int *>(abort_flag)), rank ^ 1u);
 
     if (threadIdx.x == 0) {
@@ -244,10 +280,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t policy = l2_policy_evict_normal();
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (int t = cluster; t < num_tiles && ok; t += num_clusters) {
-                const int prob = t / per_problem;
+            // One tile of job J.  J is a template parameter: with an indexed
+            // tensor map the compiler cannot tell that its address is uniform,
+            // as the copy instruction needs, and the loop that makes it so sets the
+            // pace (1024 x 4096 x 8192: 60 us against 52).
+            auto load_tile = [&](auto tag, int t) -> bool {
+                constexpr int J = decltype(tag)::value;
+                const JobArgs &job = p.job[J];
+                const int num_kb = job.num_kb * job.parts;
                 int m_blk, n_blk;
-                tile_coords(t - prob * per_problem, num_m, num_n, m_blk, n_blk);
+                tile_coords(t, job.num_m, job.num_n, m_blk, n_blk);
+                const CUtensorMap *ma = &maps.a[J][0], *mb = &maps.b[J][GATED ? rank : 0];
                 // Rows and columns beyond the matrices arrive as zeros (the
                 // maps clip), so every stage carries the same bytes.
                 const int m_mine = m_blk * PM + 128 * static_cast<int>(rank);
@@ -255,21 +298,18 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // CTA, the others from the odd one: of one weight, or (gated)
                 // of the two.
                 const int n_mine = n_blk * TILE_N + (GATED ? 0 : BN / 2 * static_cast<int>(rank));
-                for (int kb = 0; kb < num_kb; ++kb) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteProducerEmpty)) {
-                        give_up();
-                        ok = false;
-                        break;
-                    }
+                int k0 = 0;
+                for (int kb = 0; kb < num_kb; ++kb, k0 += BK) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteProducerEmpty)) return false;
                     const uint32_t full_even = mapa_shared(smem_u32(&full[stage]), 0);
                     if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE);
-                    const int part = kb >= p.num_kb ? 1 : 0;
-                    const int k0 = (kb - part * p.num_kb) * BK;
-                    const int sel = prob | part;
-                    const CUtensorMap *ma = &maps.a[sel];
-                    const CUtensorMap *mb = &maps.b[GATED ? rank : sel];
+                    if (!GATED && kb == job.num_kb) {  // the second contraction
+                        ++ma;
+                        ++mb;
+                        k0 = 0;
+                    }
                     uint8_t *da = sA + stage * A_STAGE, *db = sB + stage * Cfg::B_STAGE;
-                    if (p.a_mn) {
+                    if (job.a_mn) {
                         tma_load_2d_pair(da, ma, full_even, m_mine, k0, policy);
                         tma_load_2d_pair(da + 64 * BK * 2, ma, full_even, m_mine + 64, k0, policy);
                     } else {
@@ -279,10 +319,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int h = 0; h < NB; ++h) {
                         uint8_t *dh = db + h * Cfg::B_BLOCK;
                         const int n = n_mine + h * BLOCK_N;
-                        if (p.b_mn) {
+                        if (job.b_mn) {
 #pragma unroll
-                            for (int j = 0; j < BN / 2; j += 64)
-                                tma_load_2d_pair(dh + j * BK * 2, mb, full_even, n + j, k0, policy);
+                            for (int x = 0; x < BN / 2; x += 64)
+                                tma_load_2d_pair(dh + x * BK * 2, mb, full_even, n + x, k0, policy);
                         } else {
                             tma_load_2d_pair(dh, mb, full_even, k0, n, policy);
                         }
@@ -292,7 +332,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                         phase ^= 1u;
                     }
                 }
+                return true;
+            };
+            for (int i = 0, t; ok && (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
+                if (GATED || t < p.first[1])
+                    ok = load_tile(Index<0>{}, t);
+                else if (t < p.first[2])
+                    ok = load_tile(Index<1>{}, t - p.first[1]);
+                else
+                    ok = load_tile(Index<2>{}, t - p.first[2]);
             }
+            if (!ok) give_up();
             // This CTA's copies complete on the even CTA's barriers, which
             // only that CTA can wait on: give them time to land.
             if (!ok) spin_ns(2000000);
@@ -300,15 +350,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
     } else if (warp == 1) {
         // ---------------- MMA issuer (even CTA) ----------------
-        if (lane == 0 && rank == 0 && num_kb > 0) {
+        if (lane == 0 && rank == 0) {
             grid_dependency_wait();
+            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+            bool ok = true, issued_any = false;
             // k along the swizzle rows: 32 bytes per 16-wide step, 8-row groups
             // 1 KB apart.  Rows along them: 16 k-rows of 128 bytes per step,
             // 64-row blocks 8 KB apart.
-            const uint32_t a_step = p.a_mn ? 2048u : 32u, a_lbo = p.a_mn ? 64u * BK * 2 : 16u;
-            const uint32_t b_step = p.b_mn ? 2048u : 32u, b_lbo = p.b_mn ? 64u * BK * 2 : 16u;
-            uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
-            bool ok = true, issued_any = false;
+            uint32_t a_step = 0, a_lbo = 0, b_step = 0, b_lbo = 0, idesc = 0;
             // The MMAs of the k-block in stage st into blocks [lo, hi) of the
             // accumulator; `first` overwrites it.
             auto issue = [&](uint32_t st, bool first, int lo, int hi) {
@@ -320,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int h = lo; h < hi; ++h)
                         umma_f16_ss_pair(tmem_base + (acc + h) * BN, a_desc,
                                          smem_desc_sw128(b_base + h * Cfg::B_BLOCK + kk * b_step, b_lbo, 1024),
-                                         p.idesc, first && kk == 0 ? 0u : 1u);
+                                         idesc, first && kk == 0 ? 0u : 1u);
                 }
                 issued_any = true;
             };
@@ -375,7 +424,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (last) umma_commit_pair_multicast(&acc_full[1], 0x3);
                 return true;
             };
-            for (int t = cluster; t < num_tiles && ok; t += num_clusters) {
+            for (int i = 0, t; ok && (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
+                const JobArgs job = job_at(p, job_of(p, t));
+                const int num_kb = job.num_kb * job.parts;
+                if (num_kb == 0) continue;  // an empty sum: the epilogue's alone
+                a_step = job.a_mn ? 2048u : 32u;
+                a_lbo = job.a_mn ? 64u * BK * 2 : 16u;
+                b_step = job.b_mn ? 2048u : 32u;
+                b_lbo = job.b_mn ? 64u * BK * 2 : 16u;
+                idesc = job.idesc;
                 if (NB == 2) {
                     const int head = min(STAGES, num_kb), tail = max(head, num_kb - STAGES);
                     ok = window(0, head, true, head == num_kb) && plain(head, tail) &&
@@ -404,21 +461,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t q = warp & 3u;  // the TMEM lane quarter this warp may read
         const int side = static_cast<int>(warp - 2u) / 4;  // which of the quarter's warps
         uint32_t acc = 0, acc_phase = 0;
-        for (int t = cluster; t < num_tiles; t += num_clusters) {
-            const int prob = t / per_problem;
+        for (int i = 0, t; (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
+            const int j = job_of(p, t);
+            const JobArgs job = job_at(p, j);
+            const int num_kb = job.num_kb * job.parts;
             int m_blk, n_blk;
-            tile_coords(t - prob * per_problem, num_m, num_n, m_blk, n_blk);
+            tile_coords(t - p.first[j], job.num_m, job.num_n, m_blk, n_blk);
             const int row0 = m_blk * PM + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
             const int row = row0 + static_cast<int>(lane);
             const int n0 = n_blk * TILE_N;
-            const bool live = row < p.M;
+            const bool live = row < job.M;
             bool aborted = false;
 #pragma unroll 1
             for (int h = 0; h < NB; ++h) {
                 const uint32_t bar = acc + h;  // NB = 2: block h's own barriers
                 const int col0 = n0 + h * BLOCK_N + side * kWarpCols<GATED>;
                 Row32 res;
-                if (!GATED && p.residual.p && live && col0 < p.N) fetch_row32(p.residual, row, col0, p.N, res);
+                if (!GATED && p.residual.p && live && col0 < job.N)
+                    fetch_row32(p.residual, row, col0, job.N, res);
                 if (num_kb > 0) {
                     if (!mbar_wait(&acc_full[bar], acc_phase, abort_flag, p.status, kSiteEpilogueAccFull)) {
                         give_up();
@@ -429,15 +489,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc_fence_after_sync();
                 }
                 const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + side * kWarpCols<GATED>;
-                if (row0 < p.M)  // the whole warp: TMEM loads are warp-wide
-                    epilogue_block<GATED>(p, t_row, prob, row, col0, live, num_kb > 0, res);
+                if (row0 < job.M)  // the whole warp: TMEM loads are warp-wide
+                    epilogue_block<GATED>(p, job, t_row, row, col0, live, num_kb > 0, res);
                 tc_fence_before_sync();
                 __syncwarp();
                 if (num_kb > 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[bar]), 0));
             }
             if (aborted) break;
-            if (NB == 1) acc ^= 1u;
-            if (acc == 0) acc_phase ^= 1u;
+            if (num_kb > 0) {
+                if (NB == 1) acc ^= 1u;
+                if (acc == 0) acc_phase ^= 1u;
+            }
         }
         __syncwarp();
     }
@@ -509,27 +571,68 @@ int resident_pairs(int sm_count, int *pairs) {
     return CUDAIR_OK;
 }
 
-// Whether 256 x 512 tiles (NB = 2) beat 256 x 256 ones: waves of tiles times a
-// tile's time, in microseconds fitted on B200 (8192^3: 14 waves of 256 x 256
-// tiles 898 us against 7 of the wide ones 855 us, back to back; 2048 x 14336 x
-// 4096: 7 waves 165 us against 4 waves 198 us).  With A's rows along memory (weight
+// A tile's time in microseconds, fitted on B200: 8192^3, 14 waves of 256 x 256
+// tiles 898 us against 7 of 256 x 512 855 us, back to back; 2048 x 14336 x 4096, 7
+// waves 165 us against 4 waves 198 us.  With A's rows along memory (weight
 // gradients) the narrow tile costs more: dWg, dWu of 14336 x 4096 over 4096
-// rows, 25 waves 777 us against 13 waves 736 us.  gated keeps 256 x 256: its
-// epilogue is long enough to want two accumulators (4096 x 14336 x 4096 719
-// against 726 us, 744 against 781 us with G and U stored).
-bool wide_tiles(const Product &p, int pairs) {
-    const int64_t mt = (p.M + PM - 1) / PM * (p.form == Form::pair ? 2 : 1);
-    const double k = static_cast<double>(p.K) * (p.form == Form::sum ? 2 : 1);
-    const double w1 = static_cast<double>((mt * ((p.N + 255) / 256) + pairs - 1) / pairs);
-    const double w2 = static_cast<double>((mt * ((p.N + 511) / 512) + pairs - 1) / pairs);
-    return w2 * (0.0112 * k + 4.5) < w1 * ((p.a[0].mn ? 0.0066 : 0.0059) * k + 0.2);
+// rows, 25 waves 777 us against 13 waves 736 us.
+double tile_time(const Job &j, int nb) {
+    const double k = static_cast<double>(j.K) * j.parts;
+    return nb == 2 ? 0.0112 * k + 4.5 : (j.a[0].mn ? 0.0066 : 0.0059) * k + 0.2;
+}
+
+// How the tiles of all jobs are dealt out (see PairArgs), and how long that
+// takes.  `order` sorts the jobs by the length of their tiles.
+struct Deal {
+    int order[kMaxJobs];
+    int64_t first[kMaxJobs + 1];
+    int64_t rounds = 0;
+    double time = 0.0;
+};
+Deal deal(const Product &p, int nb, int pairs) {
+    Deal d;
+    for (int i = 0; i < p.jobs; ++i) d.order[i] = i;
+    for (int i = 1; i < p.jobs; ++i)
+        for (int k = i; k > 0 && tile_time(p.job[d.order[k]], nb) > tile_time(p.job[d.order[k - 1]], nb); --k)
+            std::swap(d.order[k], d.order[k - 1]);
+    const int64_t tile_n = static_cast<int64_t>(BN) * nb / p.tiles_of_b();
+    d.first[0] = 0;
+    for (int i = 0; i < kMaxJobs; ++i) {
+        int64_t n = 0;
+        if (i < p.jobs) {
+            const Job &j = p.job[d.order[i]];
+            n = (j.M + PM - 1) / PM * ((j.N + tile_n - 1) / tile_n);
+        }
+        d.first[i + 1] = d.first[i] + n;
+    }
+    const int64_t C = d.first[kMaxJobs] < pairs ? d.first[kMaxJobs] : pairs;
+    const int64_t n0 = d.first[1], n1 = d.first[kMaxJobs] - n0, more = n0 % C;
+    const double a = tile_time(p.job[d.order[0]], nb), b = p.jobs > 1 ? tile_time(p.job[d.order[1]], nb) : 0.0;
+    const double own = static_cast<double>(n0 / C) * a;
+    if (n1 == 0 || more == 0) {
+        d.time = own + (more ? a : 0.0) + static_cast<double>((n1 + C - 1) / C) * b;
+        return d;
+    }
+    // Level: the pairs without one more long tile do its time in short ones.
+    const int64_t level = static_cast<int64_t>((static_cast<double>(n1) - a * static_cast<double>(C - more) / b) / C);
+    d.time = 1e30;
+    for (int64_t s = level > 1 ? level - 1 : 0; s <= level + 2 && s <= (n1 + C - 1) / C; ++s) {
+        const int64_t left = n1 - s * C;  // below zero: the last round is short of that many
+        const double hi = own + a + static_cast<double>(left < -more + 1 ? s - 1 : s) * b;
+        const double lo = own + static_cast<double>(s + (left > 0 ? (left + C - more - 1) / (C - more) : 0)) * b;
+        const double t = hi > lo ? hi : lo;
+        if (t < d.time) {
+            d.time = t;
+            d.rounds = s;
+        }
+    }
+    if (d.time == 1e30) d.time = own + a;  // the short tiles end before one more long one
+    return d;
 }
 
 template <bool GATED, int NB>
 cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool pdl, cudaStream_t stream) {
-    constexpr int TILE_N = NB * (GATED ? BN / 2 : BN);
-    const int64_t tiles = static_cast<int64_t>((args.M + static_cast<int64_t>(PM) - 1) / PM) *
-                          ((args.N + static_cast<int64_t>(TILE_N) - 1) / TILE_N) * args.problems;
+    const int tiles = args.first[kMaxJobs];
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -549,42 +652,68 @@ cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool 
 
 }  // namespace
 
+int product_pair_time(const Product &p, int sm_count, double *us) {
+    int pairs = 0;
+    const int rc = resident_pairs(sm_count, &pairs);
+    if (rc != CUDAIR_OK) return rc;
+    const double narrow = deal(p, 1, pairs).time, wide = p.gated ? narrow : deal(p, 2, pairs).time;
+    *us = 6.0 + (narrow < wide ? narrow : wide);  // launch, set-up and the last epilogue
+    return CUDAIR_OK;
+}
+
 int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cudaStream_t stream) {
     int pairs = 0;
     int rc = resident_pairs(sm_count, &pairs);
     if (rc != CUDAIR_OK) return rc;
-    alignas(64) Maps maps = {};
-    const bool gated = p.form == Form::gated;
-    if (p.K > 0) {
-        const int as = p.form == Form::plain || gated ? 1 : 2, bs = p.form == Form::plain ? 1 : 2;
-        for (int i = 0; i < as; ++i)
-            if ((rc = operand_map(&maps.a[i], p.a[i], p.M, p.K, 128, p.bf16)) != CUDAIR_OK) return rc;
-        for (int i = 0; i < bs; ++i)
-            if ((rc = operand_map(&maps.b[i], p.b[i], p.N, p.K, BN / 2, p.bf16)) != CUDAIR_OK) return rc;
+    // gated keeps 256 x 256 tiles: its epilogue is long enough to want two
+    // accumulators (4096 x 14336 x 4096 719 against 726 us, 744 against 781 us with
+    // G and U stored).
+    Deal d = deal(p, 1, pairs);
+    int nb = 1;
+    if (!p.gated) {
+        const Deal wide = deal(p, 2, pairs);
+        if (wide.time < d.time) {
+            d = wide;
+            nb = 2;
+        }
     }
+    if (d.first[kMaxJobs] > INT32_MAX / 2)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: linear: %lld tiles are too many", (long long)d.first[kMaxJobs]);
+    alignas(64) Maps maps = {};
     PairArgs args = {};
-    args.M = static_cast<int>(p.M);
-    args.N = static_cast<int>(p.N);
-    args.num_kb = static_cast<int>((p.K + BK - 1) / BK);
-    args.parts = p.form == Form::sum ? 2 : 1;
-    args.problems = p.form == Form::pair ? 2 : 1;
-    args.a_mn = p.a[0].mn;
-    args.b_mn = p.b[0].mn;
-    args.idesc = idesc_f16_f32(PM, BN, p.a[0].mn, p.b[0].mn, p.bf16);
+    const int tile_n = BN * nb / p.tiles_of_b();
+    for (int i = 0; i <= kMaxJobs; ++i) args.first[i] = static_cast<int>(d.first[i]);
+    args.rounds = static_cast<int>(d.rounds);
+    for (int i = 0; i < p.jobs; ++i) {
+        const Job &j = p.job[d.order[i]];
+        JobArgs &o = args.job[i];
+        o.M = static_cast<int>(j.M);
+        o.N = static_cast<int>(j.N);
+        o.num_m = static_cast<int>((j.M + PM - 1) / PM);
+        o.num_n = static_cast<int>((j.N + tile_n - 1) / tile_n);
+        o.num_kb = static_cast<int>((j.K + BK - 1) / BK);
+        o.parts = j.parts;
+        o.a_mn = j.a[0].mn;
+        o.b_mn = j.b[0].mn;
+        o.idesc = idesc_f16_f32(PM, BN, j.a[0].mn, j.b[0].mn, p.bf16);
+        o.d = mat_of(j.d);
+        if (j.K == 0) continue;
+        for (int k = 0; k < j.parts; ++k)
+            if ((rc = operand_map(&maps.a[i][k], j.a[k], j.M, j.K, 128, p.bf16)) != CUDAIR_OK) return rc;
+        for (int k = 0; k < (p.gated ? 2 : j.parts); ++k)
+            if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, BN / 2, p.bf16)) != CUDAIR_OK) return rc;
+    }
     args.bf16 = p.bf16;
     args.act = p.act;
-    for (int i = 0; i < 2; ++i) {
-        args.d[i] = mat_of(p.d[i]);
-        args.z[i] = mat_of(p.z[i]);
-    }
+    for (int i = 0; i < 2; ++i) args.z[i] = mat_of(p.z[i]);
     args.residual = mat_of(p.residual);
     args.bias = p.bias;
     args.bias16 = p.bias16;
     args.status = status;
     const bool pdl = p.pdl();
-    const cudaError_t e = gated                 ? launch_pair<true, 1>(maps, args, pairs, pdl, stream)
-                          : wide_tiles(p, pairs) ? launch_pair<false, 2>(maps, args, pairs, pdl, stream)
-                                                : launch_pair<false, 1>(maps, args, pairs, pdl, stream);
+    const cudaError_t e = p.gated ? launch_pair<true, 1>(maps, args, pairs, pdl, stream)
+                          : nb == 2 ? launch_pair<false, 2>(maps, args, pairs, pdl, stream)
+                                    : launch_pair<false, 1>(maps, args, pairs, pdl, stream);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_pair_kernel launch");
 }
 

@@ -54,19 +54,26 @@ constexpr size_t SM_SMEM = 228 * 1024;  // per SM, 1 KB of it reserved per CTA
 static_assert(2 * MAX_STAGES * 8 + 2 * 8 + 8 <= BAR_BYTES, "barrier area");
 
 struct Maps {
-    CUtensorMap w[2], x[2];
+    CUtensorMap w[kMaxJobs][2], x[kMaxJobs][2];
+};
+
+struct JobArgs {
+    int M, N;
+    int num_kb, parts;   // k-blocks of one contraction; contractions per accumulator
+    int mt;              // rows of D per tile, a multiple of 16 (of 64 where A's rows run along memory)
+    int m_tiles, first;  // row tiles; the job's first tile
+    int w_mn, x_mn;
+    uint32_t idesc;
+    int w_early;  // B is a weight that nothing still running writes
+    Mat d;
 };
 
 struct Args {
-    int M, N;
-    int num_kb, parts, problems;
-    int mt;      // rows of D per tile, a multiple of 16 (of 64 where X is read row-major in k)
-    int m_tiles, n_tiles;
-    int split, stages;
-    int w_mn, x_mn;
-    uint32_t idesc, tmem_cols;
-    int bf16, act, w_early;
-    Mat d[2], z[2], residual;
+    JobArgs job[kMaxJobs];
+    int jobs, split, stages;
+    uint32_t x_stage, tmem_cols;  // the largest of the jobs
+    int bf16, act;
+    Mat z[2], residual;
     const void *bias;
     int bias16;
     unsigned int *status;
@@ -161,7 +168,7 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t *smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);  // the same offset in every rank
 
-    const uint32_t x_stage = static_cast<uint32_t>(p.mt) * BK * 2;
+    const uint32_t x_stage = p.x_stage;
     const int STAGES = p.stages;
     uint8_t *sW = smem;
     uint8_t *sX = smem + STAGES * W_TILES * W_TILE;
@@ -177,28 +184,32 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     const uint32_t warp = warp_id(), lane = lane_id();
     const int rank = static_cast<int>(blockIdx.x % p.split);
     int tile = static_cast<int>(blockIdx.x / p.split);
-    const int per_problem = p.m_tiles * p.n_tiles;
-    const int prob = tile / per_problem;
-    tile -= prob * per_problem;
-    const int m0 = tile % p.m_tiles * p.mt, n0 = tile / p.m_tiles * NT;
-    const int rows = min(p.mt, p.M - m0);
-    const int total_kb = p.num_kb * p.parts;
+    int ji = 0;
+    if (p.jobs > 1 && tile >= p.job[1].first) ji = p.jobs > 2 && tile >= p.job[2].first ? 2 : 1;
+    const JobArgs job = ji == 0 ? p.job[0] : ji == 1 ? p.job[1] : p.job[2];  // fixed places: in registers
+    tile -= job.first;
+    const int mt = job.mt;
+    const int m0 = tile % job.m_tiles * mt, n0 = tile / job.m_tiles * NT;
+    const int rows = min(mt, job.M - m0);
+    const int total_kb = job.num_kb * job.parts;
     const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * rank / p.split);
     const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (rank + 1) / p.split);
 
     if (threadIdx.x == 64) grid_launch_dependents();  // cudair_set_gemm_pdl
 
     const int head = min(kb1 - kb0, STAGES);
+    const int part_kb = job.num_kb, w_mn = job.w_mn, x_mn = job.x_mn;
+    const CUtensorMap *map_w = &maps.w[ji][0], *map_x = &maps.x[ji][0];
     const uint64_t policy = l2_policy_evict_normal();
     auto load_w = [&](int kb, int st) {
-        const int sel = prob | (kb >= p.num_kb ? 1 : 0);
-        const int k0 = (kb >= p.num_kb ? kb - p.num_kb : kb) * BK;
-        mbar_arrive_expect_tx(&full[st], W_TILES * W_TILE + x_stage);
+        const int part = kb >= part_kb ? 1 : 0;
+        const int k0 = (kb - part * part_kb) * BK;
+        mbar_arrive_expect_tx(&full[st], W_TILES * W_TILE + static_cast<uint32_t>(mt) * BK * 2);
 #pragma unroll
         for (int i = 0; i < W_TILES; ++i) {
-            const CUtensorMap *mw = &maps.w[GATED ? i : sel];
+            const CUtensorMap *mw = map_w + (GATED ? i : part);
             uint8_t *dst = sW + (st * W_TILES + i) * W_TILE;
-            if (p.w_mn) {
+            if (w_mn) {
                 tma_load_2d(dst, mw, &full[st], n0, k0, policy);
                 tma_load_2d(dst + W_BOX, mw, &full[st], n0 + 64, k0, policy);
             } else {
@@ -207,14 +218,14 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
         }
     };
     auto load_x = [&](int kb, int st) {
-        const int sel = prob | (kb >= p.num_kb ? 1 : 0);
-        const int k0 = (kb >= p.num_kb ? kb - p.num_kb : kb) * BK;
+        const int part = kb >= part_kb ? 1 : 0;
+        const int k0 = (kb - part * part_kb) * BK;
         uint8_t *dst = sX + st * x_stage;
-        if (p.x_mn) {
-            for (int j = 0; j < p.mt; j += 64)
-                tma_load_2d(dst + j * (BK * 2), &maps.x[sel], &full[st], m0 + j, k0, policy);
+        if (x_mn) {
+            for (int j = 0; j < mt; j += 64)
+                tma_load_2d(dst + j * (BK * 2), map_x + part, &full[st], m0 + j, k0, policy);
         } else {
-            tma_load_2d(dst, &maps.x[sel], &full[st], k0, m0, policy);
+            tma_load_2d(dst, map_x + part, &full[st], k0, m0, policy);
         }
     };
 
@@ -230,12 +241,12 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
-        if (!p.w_early) grid_dependency_wait();
+        if (!job.w_early) grid_dependency_wait();
         for (int i = 0; i < head; ++i) {
             load_w(kb0 + i, i);
-            if (!p.w_early) load_x(kb0 + i, i);
+            if (!job.w_early) load_x(kb0 + i, i);
         }
-        if (p.w_early) {
+        if (job.w_early) {
             grid_dependency_wait();
             for (int i = 0; i < head; ++i) load_x(kb0 + i, i);
         }
@@ -284,8 +295,9 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
         // ---------------- MMA issuer ----------------
         if (lane == 0 && kb1 > kb0) {
             grid_dependency_wait();
-            const uint32_t w_step = p.w_mn ? 2048u : 32u, w_lbo = p.w_mn ? W_BOX : 16u;
-            const uint32_t x_step = p.x_mn ? 2048u : 32u, x_lbo = p.x_mn ? W_BOX : 16u;
+            const uint32_t w_step = w_mn ? 2048u : 32u, w_lbo = w_mn ? W_BOX : 16u;
+            const uint32_t x_step = x_mn ? 2048u : 32u, x_lbo = x_mn ? W_BOX : 16u;
+            const uint32_t idesc = job.idesc;
             int st = 0;
             uint32_t phase = 0;
             bool ok = true, issued_any = false;
@@ -302,9 +314,9 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
                     const uint64_t x_desc = smem_desc_sw128(x_base + kk * x_step, x_lbo, 1024);
 #pragma unroll
                     for (int i = 0; i < W_TILES; ++i)
-                        umma_f16_ss(tmem_base + i * p.mt,
+                        umma_f16_ss(tmem_base + i * mt,
                                     smem_desc_sw128(w_base + i * W_TILE + kk * w_step, w_lbo, 1024), x_desc,
-                                    p.idesc, (kb - kb0) | kk ? 1u : 0u);
+                                    idesc, (kb - kb0) | kk ? 1u : 0u);
                 }
                 issued_any = true;
                 umma_commit(&empty[st]);
@@ -337,15 +349,15 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
 #pragma unroll 1
                     for (int c = half * 16; c < rows; c += EPI_WARPS * 4) {
                         uint32_t r[16];
-                        tmem_ld_32x32b_x16(tmem_base + ((q * 32u) << 16) + i * p.mt + c, r);
+                        tmem_ld_32x32b_x16(tmem_base + ((q * 32u) << 16) + i * mt + c, r);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) mine[(i * p.mt + c + j) * NT] = __uint_as_float(r[j]);
+                        for (int j = 0; j < 16; ++j) mine[(i * mt + c + j) * NT] = __uint_as_float(r[j]);
                     }
             }
         } else {  // an empty run: K = 0, or fewer k-blocks than ranks
             for (int i = 0; i < W_TILES; ++i)
-                for (int c = half; c < rows; c += EPI_WARPS / 4) mine[(i * p.mt + c) * NT] = 0.0f;
+                for (int c = half; c < rows; c += EPI_WARPS / 4) mine[(i * mt + c) * NT] = 0.0f;
         }
         __syncwarp();
         tc_fence_before_sync();
@@ -361,13 +373,13 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     // four columns a lane.
     grid_dependency_wait();
     const int col = n0 + static_cast<int>(lane) * 4;
-    if (col < p.N) {
+    if (col < job.N) {
         const bool bf16 = p.bf16 != 0;
         float bias[4] = {};
         if (p.bias) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (col + j < p.N)
+                if (col + j < job.N)
                     bias[j] = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[col + j], bf16)
                                        : static_cast<const float *>(p.bias)[col + j];
         }
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
             if (p.residual.p) {
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b)
-                    res[b] = fetch4(p.residual, m0 + rank + min(k0 + b, own - 1) * p.split, col, p.N);
+                    res[b] = fetch4(p.residual, m0 + rank + min(k0 + b, own - 1) * p.split, col, job.N);
             }
 #pragma unroll
             for (int r = 0; r < MAX_SPLIT; ++r)
@@ -392,7 +404,7 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
 #pragma unroll
                         for (int i = 0; i < W_TILES; ++i) {
                             const int c = rank + min(k0 + b, own - 1) * p.split;
-                            t[b * W_TILES + i][r] = ld_cluster_f4(from + (i * p.mt + c) * (NT * 4));
+                            t[b * W_TILES + i][r] = ld_cluster_f4(from + (i * mt + c) * (NT * 4));
                         }
                 }
 #pragma unroll
@@ -415,8 +427,8 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
                 float out[4];
                 if (GATED) {
                     if (p.z[0].p) {
-                        store4(p.z[0], row, col, p.N, bf16, v[0]);
-                        store4(p.z[1], row, col, p.N, bf16, v[W_TILES - 1]);
+                        store4(p.z[0], row, col, job.N, bf16, v[0]);
+                        store4(p.z[1], row, col, job.N, bf16, v[W_TILES - 1]);
                     }
                     with_act(p.act, [&](auto tag) {
 #pragma unroll
@@ -426,14 +438,14 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[0][j] += bias[j];
-                    if (p.z[0].p) store4(p.z[0], row, col, p.N, bf16, v[0]);
+                    if (p.z[0].p) store4(p.z[0], row, col, job.N, bf16, v[0]);
                     with_act(p.act, [&](auto tag) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) out[j] = act_value<decltype(tag)::value>(v[0][j]);
                     });
                     if (p.residual.p) add4(res[b], p.residual.f32, bf16, out);
                 }
-                store4(p.d[prob], row, col, p.N, bf16, out);
+                store4(job.d, row, col, job.N, bf16, out);
             }
         }
     }
@@ -535,88 +547,108 @@ int prepare_device(const Device **out) {
 // exceed one wave above M = 96 (128 x 32768 x 2048: 36.6 against 32.6 us);
 // above, where the tiles leave room to split at all (1024 x 1024 x 4096 18.0
 // against 26.0 us; 1024 x 4096 x 4096, 256 tiles, 44.7 against 28.6 us).
+// Several jobs (the gradients of a call) share one grid; they go to the pair
+// kernel when one of them would alone.
 int split_plan(const Product &p, SplitPlan *plan) {
     using namespace split;
     const Device *dev = nullptr;
     const int rc = prepare_device(&dev);
     if (rc != CUDAIR_OK) return rc;
-    const int w_tiles = p.form == Form::gated ? 2 : 1;
-    const int64_t n_tiles = (p.N + NT - 1) / NT * (p.form == Form::pair ? 2 : 1);
-    const int64_t kb = (p.K + BK - 1) / BK * (p.form == Form::sum ? 2 : 1);
-    auto tiles = [&](int mt) { return (p.M + mt - 1) / mt * n_tiles; };
+    const int w_tiles = p.tiles_of_b();
     // The largest split whose clusters all fit, with one or two CTAs per SM (0: none).
-    auto fits = [&](int64_t t, int two) {
+    auto fits = [&](int64_t tiles, int64_t kb, int two) {
         for (int s = static_cast<int>(std::min<int64_t>(MAX_SPLIT, std::max<int64_t>(kb, 1))); s > 0; --s)
-            if (t <= dev->clusters[two][s]) return s;
+            if (tiles <= dev->clusters[two][s]) return s;
         return 0;
     };
-    // 64 rows at a time where A is read with rows along memory.
-    const int unit = p.a[0].mn ? 64 : 16;
-    int mt = static_cast<int>(std::min<int64_t>(128, (p.M + unit - 1) / unit * unit));
-    if (mt > 64 && fits(tiles(64), 0) >= 4) mt = 64;
-    const int64_t t = tiles(mt);
-    const int one = fits(t, 0);
     plan->split = 0;
-    if (p.M > 128 ? one < 2 : p.M > 96 && one < 1) return CUDAIR_OK;
-    const bool deep = w_tiles * static_cast<int>(W_TILE) + mt * BK * 2 > 28 * 1024;  // a stage: under four in half an SM
-    int split = std::max(one, 1), two = deep ? 0 : 1;
-    if (one <= 2 && kb >= 24 * split && !(w_tiles == 2 && mt > 64)) {
-        split = std::max(fits(t, 1), 1);
-        two = 1;
+    int64_t total = 0, most_kb = 0;
+    int most_mt = 0;
+    for (int i = 0; i < p.jobs; ++i) {
+        const Job &j = p.job[i];
+        const int64_t n_tiles = (j.N + NT - 1) / NT, kb = (j.K + BK - 1) / BK * j.parts;
+        auto tiles = [&](int mt) { return (j.M + mt - 1) / mt * n_tiles; };
+        const int unit = j.a[0].mn ? 64 : 16;
+        int mt = static_cast<int>(std::min<int64_t>(128, (j.M + unit - 1) / unit * unit));
+        const int one = fits(tiles(mt), kb, 0);
+        if (j.M > 128 ? one < 2 : j.M > 96 && one < 1) return CUDAIR_OK;
+        if (mt > 64 && p.jobs == 1 && fits(tiles(64), kb, 0) >= 4) mt = 64;
+        plan->mt[i] = mt;
+        most_mt = std::max(most_mt, mt);
+        most_kb = std::max(most_kb, kb);
+        total += tiles(mt);
     }
+    const int one = fits(total, most_kb, 0);
+    // A stage of which fewer than four fit half an SM.
+    const bool deep = w_tiles * static_cast<int>(W_TILE) + most_mt * BK * 2 > 28 * 1024;
+    const bool can_share = !(w_tiles == 2 && most_mt > 64);
+    int split = std::max(one, 1), two = deep ? 0 : 1;
     // Where even whole tiles exceed one wave (wide N), two CTAs per SM overlap
     // one's join with the other's stream.
-    if (one == 0 && !(w_tiles == 2 && mt > 64)) two = 1;
-    plan->mt = mt;
+    if (can_share && (one == 0 || (one <= 2 && most_kb >= 24 * split))) {
+        split = std::max(fits(total, most_kb, 1), 1);
+        two = 1;
+    }
+    if (total * split > INT32_MAX)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: linear: %lld tiles are too many", (long long)total);
     plan->split = split;
-    plan->stages = std::min(MAX_STAGES, static_cast<int>((kBudget[two] - fixed_bytes()) / ring_bytes(w_tiles, mt, 1)));
+    // Launch, set-up and join, then a CTA's k-blocks at the pace that its share
+    // of an SM and of HBM allows (tiles of 128 rows: 16 k-blocks a CTA with 128 CTAs 13.7
+    // us, with 256 CTAs 18.9 us).
+    const double ctas = static_cast<double>(total * split), places = dev->clusters[two][split] * split;
+    const double per_sm = std::min(ctas, places) / dev->clusters[0][1];
+    plan->time = 5.5 + static_cast<double>((most_kb + split - 1) / split) * (0.3 + 0.29 * per_sm) *
+                           std::max(1.0, ctas / places);
+    plan->stages =
+        std::min(MAX_STAGES, static_cast<int>((kBudget[two] - fixed_bytes()) / ring_bytes(w_tiles, most_mt, 1)));
     return CUDAIR_OK;
 }
 
 int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *status, cudaStream_t stream) {
     using namespace split;
-    const Device *dev = nullptr;
-    int rc = prepare_device(&dev);
-    if (rc != CUDAIR_OK) return rc;
-    const bool gated = p.form == Form::gated;
-    const int w_tiles = gated ? 2 : 1;
+    const int w_tiles = p.tiles_of_b();
     alignas(64) split::Maps maps = {};
-    if (p.K > 0) {
-        const int as = p.form == Form::plain || gated ? 1 : 2, bs = p.form == Form::plain ? 1 : 2;
-        for (int i = 0; i < bs; ++i)
-            if ((rc = operand_map(&maps.w[i], p.b[i], p.N, p.K, NT, p.bf16)) != CUDAIR_OK) return rc;
-        for (int i = 0; i < as; ++i)
-            if ((rc = operand_map(&maps.x[i], p.a[i], p.M, p.K, static_cast<uint32_t>(plan.mt), p.bf16)) !=
-                CUDAIR_OK)
+    split::Args args = {};
+    int rc = CUDAIR_OK, tiles = 0, most_mt = 0;
+    for (int i = 0; i < p.jobs; ++i) {
+        const Job &j = p.job[i];
+        split::JobArgs &o = args.job[i];
+        o.M = static_cast<int>(j.M);
+        o.N = static_cast<int>(j.N);
+        o.num_kb = static_cast<int>((j.K + split::BK - 1) / split::BK);
+        o.parts = j.parts;
+        o.mt = plan.mt[i];
+        o.m_tiles = static_cast<int>((j.M + o.mt - 1) / o.mt);
+        o.first = tiles;
+        tiles += o.m_tiles * static_cast<int>((j.N + NT - 1) / NT);
+        most_mt = std::max(most_mt, o.mt);
+        o.w_mn = j.b[0].mn;
+        o.x_mn = j.a[0].mn;
+        o.idesc = idesc_f16_f32(NT, static_cast<uint32_t>(o.mt), j.b[0].mn, j.a[0].mn, p.bf16);
+        o.w_early = j.b_weights && p.weights_early();
+        o.d = mat_of(j.d);
+        if (j.K == 0) continue;
+        for (int k = 0; k < (p.gated ? 2 : j.parts); ++k)
+            if ((rc = operand_map(&maps.w[i][k], j.b[k], j.N, j.K, NT, p.bf16)) != CUDAIR_OK) return rc;
+        for (int k = 0; k < j.parts; ++k)
+            if ((rc = operand_map(&maps.x[i][k], j.a[k], j.M, j.K, static_cast<uint32_t>(o.mt), p.bf16)) != CUDAIR_OK)
                 return rc;
     }
-    split::Args args = {};
-    args.M = static_cast<int>(p.M);
-    args.N = static_cast<int>(p.N);
-    args.num_kb = static_cast<int>((p.K + split::BK - 1) / split::BK);
-    args.parts = p.form == Form::sum ? 2 : 1;
-    args.problems = p.form == Form::pair ? 2 : 1;
-    args.mt = plan.mt;
-    args.m_tiles = static_cast<int>((p.M + plan.mt - 1) / plan.mt);
-    args.n_tiles = static_cast<int>((p.N + NT - 1) / NT);
+    args.jobs = p.jobs;
     args.split = plan.split;
     args.stages = plan.stages;
-    args.w_mn = p.b[0].mn;
-    args.x_mn = p.a[0].mn;
-    args.idesc = idesc_f16_f32(NT, static_cast<uint32_t>(plan.mt), p.b[0].mn, p.a[0].mn, p.bf16);
-    args.tmem_cols = tmem_cols_for(w_tiles, plan.mt);
+    args.x_stage = static_cast<uint32_t>(most_mt) * split::BK * 2;
+    args.tmem_cols = tmem_cols_for(w_tiles, most_mt);
     args.bf16 = p.bf16;
     args.act = p.act;
-    args.w_early = p.weights_early();
-    for (int i = 0; i < 2; ++i) {
-        args.d[i] = mat_of(p.d[i]);
-        args.z[i] = mat_of(p.z[i]);
-    }
+    for (int i = 0; i < 2; ++i) args.z[i] = mat_of(p.z[i]);
     args.residual = mat_of(p.residual);
     args.bias = p.bias;
     args.bias16 = p.bias16;
     args.status = status;
-    const size_t smem = std::max(fixed_bytes() + ring_bytes(w_tiles, plan.mt, plan.stages), smem_floor(args.tmem_cols));
+    // Up to 32 rows the join is short and four warps do it (eight cost 0.3 us
+    // more, 1 x 4096 x 4096); above, eight (gated 64 x 14336 x 4096: 46.0 -> 45.2 us).
+    const bool many = most_mt > 32;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -625,19 +657,17 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(args.m_tiles) * args.n_tiles * args.problems * plan.split, 1, 1);
-    // Up to 32 rows the join is short and four warps do it (eight cost 0.3 us
-    // more, 1 x 4096 x 4096); above, eight (gated 64 x 14336 x 4096: 46.0 -> 45.2 us).
-    const bool many = plan.mt > 32;
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles) * plan.split, 1, 1);
     cfg.blockDim = dim3(static_cast<unsigned>(threads(many ? 8 : 4)), 1, 1);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes =
+        std::max(fixed_bytes() + ring_bytes(w_tiles, most_mt, plan.stages), smem_floor(args.tmem_cols));
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = p.pdl() ? 2 : 1;
-    const cudaError_t e = gated ? (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<true, 8>, maps, args)
-                                        : cudaLaunchKernelEx(&cfg, product_split_kernel<true, 4>, maps, args))
-                                : (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<false, 8>, maps, args)
-                                        : cudaLaunchKernelEx(&cfg, product_split_kernel<false, 4>, maps, args));
+    const cudaError_t e = p.gated ? (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<true, 8>, maps, args)
+                                          : cudaLaunchKernelEx(&cfg, product_split_kernel<true, 4>, maps, args))
+                                  : (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<false, 8>, maps, args)
+                                          : cudaLaunchKernelEx(&cfg, product_split_kernel<false, 4>, maps, args));
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_split_kernel launch");
 }
 
