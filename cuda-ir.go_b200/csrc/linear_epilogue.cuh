@@ -28,22 +28,38 @@ namespace ffn {
 // length is the epilogue's: with expf, an IEEE division and normcdff a
 // 256-column tile took 18 us (silu, 256 x 1024 outputs; 40 us where the
 // division leaves its fast path) against 2 us without an activation.  So the
-// exponential and the reciprocal are the hardware's (__expf: 2^-22 plus
-// |z| 2^-24 of the value; __fdividef: two units, and 0 for a denominator
-// above 2^126, where the quotient is below 2^-126 anyway).
+// power of two and the reciprocal are one hardware instruction each: 2^-22 of
+// the value, with the argument's rounding |z| 2^-23 more for e^z; results below
+// 2^-126 become 0.
 
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluB = 0.044715f;
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float sigmoid(float z) { return rcp_fast(1.0f + exp2_fast(-kLog2E * z)); }
+// sigmoid(2y) of gelu_tanh, from z and z^2: the constants of 2y and of e^-2y in one.
+__device__ __forceinline__ float gelu_tanh_sigmoid(float z, float z2) {
+    return rcp_fast(1.0f + exp2_fast(z * fmaf(-kLog2E * kGeluC * kGeluB, z2, -kLog2E * kGeluC)));
+}
 
 // P(z) and E = e^(-z^2 / 2).  The tail is Abramowitz and Stegun's 7.1.26 for
 // erfc(x), x = |z| / sqrt(2): a polynomial in t = 1 / (1 + p x) times e^(-x^2),
 // off by at most 1.5e-7 (so P by 0.75e-7, an fp32 rounding of 1).
 __device__ __forceinline__ void normal_integral(float z, float &P, float &E) {
     const float x = fabsf(z) * 0.7071067811865476f;
-    E = __expf(-0.5f * z * z);
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    E = exp2_fast(-0.5f * kLog2E * z * z);
+    const float t = rcp_fast(fmaf(0.3275911f, x, 1.0f));
     float h = fmaf(t, 1.061405429f, -1.453152027f);
     h = fmaf(t, h, 1.421413741f);
     h = fmaf(t, h, -0.284496736f);
@@ -61,7 +77,7 @@ __device__ __forceinline__ float act_value(float z) {
         normal_integral(z, P, E);
         return z * P;
     }
-    if (ACT == CUDAIR_ACT_GELU_TANH) return z * sigmoid(kGeluC * (z + kGeluB * z * z * z));
+    if (ACT == CUDAIR_ACT_GELU_TANH) return z * gelu_tanh_sigmoid(z, z * z);
     return z;
 }
 
@@ -82,11 +98,11 @@ __device__ __forceinline__ void act_both(float z, float &value, float &grad) {
         grad = P + z * (0.3989422804014327f * E);
     } else if (ACT == CUDAIR_ACT_GELU_TANH) {
         const float z2 = z * z;
-        const float s = sigmoid(kGeluC * (z + kGeluB * z * z2));
+        const float s = gelu_tanh_sigmoid(z, z2);
         value = z * s;
         // s (1 - s) is zero where s is 0 or 1; z^2 may be infinite there.
-        const float w = s * (1.0f - s);
-        grad = w == 0.0f ? s : s + z * w * (kGeluC * (1.0f + 3.0f * kGeluB * z2));
+        const float w = s - s * s;
+        grad = w == 0.0f ? s : s + w * (z * fmaf(3.0f * kGeluB * kGeluC, z2, kGeluC));
     } else {
         value = z;
         grad = 1.0f;
@@ -273,6 +289,35 @@ __device__ __forceinline__ void add_row32(const Row32 &r, bool f32, bool bf16, f
             unpack16(r.w[j], bf16, lo, hi);
             v[2 * j] += lo;
             v[2 * j + 1] += hi;
+        }
+    }
+}
+
+// Adds 32 values that every row shares, from a 16-byte aligned vector.
+__device__ __forceinline__ void add_row32_uniform(const void *p, bool is16, bool bf16, int col, float (&v)[32]) {
+    if (is16) {
+        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + col);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint4 w = q[j];
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float lo, hi;
+                unpack16(u[k], bf16, lo, hi);
+                v[8 * j + 2 * k] += lo;
+                v[8 * j + 2 * k + 1] += hi;
+            }
+        }
+    } else {
+        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + col);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float4 f = q[j];
+            v[4 * j] += f.x;
+            v[4 * j + 1] += f.y;
+            v[4 * j + 2] += f.z;
+            v[4 * j + 3] += f.w;
         }
     }
 }

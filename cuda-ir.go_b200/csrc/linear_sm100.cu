@@ -97,10 +97,10 @@ struct PairArgs {
     JobArgs job[kMaxJobs];
     int first[kMaxJobs + 1];  // a job's first tile; the end
     int rounds;
-    int bf16, act;
+    int act;
     Mat z[2], residual;
     const void *bias;
-    int bias16;
+    int bias16, bias_wide;  // bias_wide: 16-byte aligned
     unsigned int *status;
 };
 
@@ -172,10 +172,9 @@ constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
 // where they start in TMEM.  `next` holds the residual's first 32 columns,
 // requested before the accumulator was waited for; each further 32 are
 // requested while the ones before them are worked on.
-template <bool GATED>
+template <bool GATED, bool bf16>
 __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row, int n0, bool live,
                                                bool any, Row32 &next) {
-    const bool bf16 = p.bf16 != 0;
 #pragma unroll 1
     for (int c = 0; c < kWarpCols<GATED>; c += 32) {
         const int col = n0 + c;
@@ -195,14 +194,20 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
             });
         } else {
             if (p.bias) {
-                // Lane l reads column l's bias; a shuffle hands it on.
-                float b = 0.0f;
-                const int bc = col + static_cast<int>(lane_id());
-                if (bc < job.N)
-                    b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
-                                 : static_cast<const float *>(p.bias)[bc];
+                // Every lane adds the same 32 values: whole blocks by uniform
+                // 16-byte loads, a last one that ends inside the 32 through a
+                // shuffle of lane l's column l.
+                if (p.bias_wide && col + 32 <= job.N) {
+                    add_row32_uniform(p.bias, p.bias16, bf16, col, v);
+                } else {
+                    float b = 0.0f;
+                    const int bc = col + static_cast<int>(lane_id());
+                    if (bc < job.N)
+                        b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
+                                     : static_cast<const float *>(p.bias)[bc];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
+                    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
+                }
             }
             if (p.z[0].p && live) store_row32(p.z[0], row, col, job.N, bf16, v);
             if (p.act != CUDAIR_ACT_NONE)
@@ -220,7 +225,7 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
     }
 }
 
-template <bool GATED, int NB>
+template <bool GATED, int NB, bool BF16>
 __global__ void __launch_bounds__(THREADS, 1)
     product_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ PairArgs p) {
     using Cfg = PairCfg<NB>;
@@ -490,7 +495,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + side * kWarpCols<GATED>;
                 if (row0 < job.M)  // the whole warp: TMEM loads are warp-wide
-                    epilogue_block<GATED>(p, job, t_row, row, col0, live, num_kb > 0, res);
+                    epilogue_block<GATED, BF16>(p, job, t_row, row, col0, live, num_kb > 0, res);
                 tc_fence_before_sync();
                 __syncwarp();
                 if (num_kb > 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[bar]), 0));
@@ -533,9 +538,9 @@ namespace {
 std::mutex g_pair_mu;
 int g_pairs[64];  // CTA pairs resident at once, per device (0: not asked yet)
 
-template <bool GATED, int NB>
+template <bool GATED, int NB, bool BF16>
 cudaError_t prepare_kernel(int sm_count, int *clusters) {
-    cudaError_t e = cudaFuncSetAttribute(product_pair_kernel<GATED, NB>,
+    cudaError_t e = cudaFuncSetAttribute(product_pair_kernel<GATED, NB, BF16>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(PairCfg<NB>::SMEM));
     if (e != cudaSuccess) return e;
@@ -550,7 +555,7 @@ cudaError_t prepare_kernel(int sm_count, int *clusters) {
     cfg.dynamicSmemBytes = PairCfg<NB>::SMEM;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaOccupancyMaxActiveClusters(clusters, product_pair_kernel<GATED, NB>, &cfg);
+    return cudaOccupancyMaxActiveClusters(clusters, product_pair_kernel<GATED, NB, BF16>, &cfg);
 }
 
 int resident_pairs(int sm_count, int *pairs) {
@@ -560,9 +565,12 @@ int resident_pairs(int sm_count, int *pairs) {
     std::lock_guard<std::mutex> lk(g_pair_mu);  // dev is in 0..63: the device check passed
     if (g_pairs[dev] == 0) {
         int n = 0;
-        if ((e = prepare_kernel<false, 1>(sm_count, &n)) != cudaSuccess ||
-            (e = prepare_kernel<false, 2>(sm_count, &n)) != cudaSuccess ||
-            (e = prepare_kernel<true, 1>(sm_count, &n)) != cudaSuccess)
+        if ((e = prepare_kernel<false, 1, false>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<false, 1, true>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<false, 2, false>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<false, 2, true>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<true, 1, false>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<true, 1, true>(sm_count, &n)) != cudaSuccess)
             return cuda_error(e, "product_pair_kernel set-up");
         if (n < 1) return set_error(CUDAIR_ERR_CUDA, "cudair: no CTA pair of the linear kernels fits this device");
         g_pairs[dev] = n;
@@ -631,7 +639,8 @@ Deal deal(const Product &p, int nb, int pairs) {
 }
 
 template <bool GATED, int NB>
-cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool pdl, cudaStream_t stream) {
+cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool bf16, bool pdl,
+                        cudaStream_t stream) {
     const int tiles = args.first[kMaxJobs];
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -647,7 +656,8 @@ cudaError_t launch_pair(const Maps &maps, const PairArgs &args, int pairs, bool 
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NB>, maps, args);
+    return bf16 ? cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NB, true>, maps, args)
+                : cudaLaunchKernelEx(&cfg, product_pair_kernel<GATED, NB, false>, maps, args);
 }
 
 }  // namespace
@@ -703,17 +713,17 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
         for (int k = 0; k < (p.gated ? 2 : j.parts); ++k)
             if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, BN / 2, p.bf16)) != CUDAIR_OK) return rc;
     }
-    args.bf16 = p.bf16;
     args.act = p.act;
     for (int i = 0; i < 2; ++i) args.z[i] = mat_of(p.z[i]);
     args.residual = mat_of(p.residual);
     args.bias = p.bias;
     args.bias16 = p.bias16;
+    args.bias_wide = (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
     args.status = status;
     const bool pdl = p.pdl();
-    const cudaError_t e = p.gated ? launch_pair<true, 1>(maps, args, pairs, pdl, stream)
-                          : nb == 2 ? launch_pair<false, 2>(maps, args, pairs, pdl, stream)
-                                    : launch_pair<false, 1>(maps, args, pairs, pdl, stream);
+    const cudaError_t e = p.gated ? launch_pair<true, 1>(maps, args, pairs, p.bf16, pdl, stream)
+                          : nb == 2 ? launch_pair<false, 2>(maps, args, pairs, p.bf16, pdl, stream)
+                                    : launch_pair<false, 1>(maps, args, pairs, p.bf16, pdl, stream);
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_pair_kernel launch");
 }
 
