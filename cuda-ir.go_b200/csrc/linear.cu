@@ -340,16 +340,35 @@ OutMat out_mat(void *p, int64_t ld, bool f32) {
 
 }  // namespace
 
-// One launch, by the kernel that suits it.
+namespace {
+
+// One launch, by the kernel that is the faster one by their estimates.  Up to
+// 64 rows that is the split kernel: the pair kernel's 256-row tiles would read the
+// weights at the pace of few SMs (gated 1 x 4672 x 7296: 124 against 26 us).
 struct Launch {
     SplitPlan plan;
+    bool split = true;
     double time = 0.0;
 };
-static int plan_launch(const Product &p, int sm_count, Launch *l) {
+int plan_launch(const Product &p, int sm_count, Launch *l) {
     CUDAIR_TRY(split_plan(p, &l->plan));
     l->time = l->plan.time;
-    return l->plan.split > 0 ? CUDAIR_OK : product_pair_time(p, sm_count, &l->time);
+    bool few = true;
+    for (int i = 0; i < p.jobs; ++i) few = few && p.job[i].M <= 64;
+    if (few) return CUDAIR_OK;
+    double pair = 0.0;
+    CUDAIR_TRY(product_pair_time(p, sm_count, &pair));
+    if (pair < l->time) {
+        l->split = false;
+        l->time = pair;
+    }
+    return CUDAIR_OK;
 }
+int start(const Product &p, const Launch &l, int sm_count, unsigned int *status, cudaStream_t stream) {
+    return l.split ? product_split_launch(p, l.plan, status, stream) : product_pair_launch(p, sm_count, status, stream);
+}
+
+}  // namespace
 
 int product_launch(const Product &p, cudaStream_t stream) {
     unsigned int *status = nullptr;
@@ -357,31 +376,27 @@ int product_launch(const Product &p, cudaStream_t stream) {
     CUDAIR_TRY(wait_status_current_device(&status));  // with the device and context checks
     CUDAIR_TRY(sm_count_current_device(&sms));
     Launch all;
-    if (p.jobs == 1) {
-        CUDAIR_TRY(split_plan(p, &all.plan));
-    } else {
+    CUDAIR_TRY(plan_launch(p, sms, &all));
+    if (p.jobs > 1) {
         // A call's gradients share one launch (4096 x 14336 x 4096: linear 752 ->
-        // 722 us, gated 1402 -> 1360 us; 301 x 515 x 1029 25.8 -> 15.0 us), unless
-        // the first, whose contraction may be the longest, has few tiles that
-        // the split kernel would cut: then it runs by itself, and the weights'
-        // gradients after it (gated 203 x 1731 x 777: 46 us together, 25 us in two).
+        // 711 us, gated 1402 -> 1335 us; 301 x 515 x 1029 26 -> 15 us), unless the
+        // first, whose contraction may be the longest, has few tiles that the
+        // split kernel would cut: then it runs by itself, and the weights' gradients after it
+        // (gated 203 x 1731 x 777: 46 us together, 25 us in two).
         Product first = p, rest = p;
         first.jobs = 1;
         rest.jobs = p.jobs - 1;
         for (int i = 0; i < rest.jobs; ++i) rest.job[i] = p.job[i + 1];
         rest.chained = true;
         Launch one, two;
-        CUDAIR_TRY(plan_launch(p, sms, &all));
         CUDAIR_TRY(plan_launch(first, sms, &one));
         CUDAIR_TRY(plan_launch(rest, sms, &two));
         if (one.time + two.time < all.time) {
-            CUDAIR_TRY(product_launch(first, stream));
-            return rest.jobs == 1 || two.plan.split > 0 ? product_launch(rest, stream)
-                                                        : product_pair_launch(rest, sms, status, stream);
+            CUDAIR_TRY(start(first, one, sms, status, stream));
+            return start(rest, two, sms, status, stream);
         }
     }
-    if (all.plan.split > 0) return product_split_launch(p, all.plan, status, stream);
-    return product_pair_launch(p, sms, status, stream);
+    return start(p, all, sms, status, stream);
 }
 
 }  // namespace ffn

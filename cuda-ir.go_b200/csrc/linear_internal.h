@@ -75,10 +75,8 @@ struct SplitPlan {
     int mt[kMaxJobs] = {}, split = 0, stages = 0;
     double time = 0.0;  // estimated, in microseconds
 };
-int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *status, cudaStream_t stream);
-// How the split kernel should run these products; plan->split is 0 where the
-// pair kernel is the faster one.
 int split_plan(const Product &p, SplitPlan *plan);
+int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *status, cudaStream_t stream);
 
 // Shared by the two: an operand's tensor map, with boxes of 64 k x box_rows
 // rows where k runs along memory, else of 64 rows x 64 k; 128-byte swizzle.

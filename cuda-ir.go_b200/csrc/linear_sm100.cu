@@ -667,7 +667,7 @@ int product_pair_time(const Product &p, int sm_count, double *us) {
     const int rc = resident_pairs(sm_count, &pairs);
     if (rc != CUDAIR_OK) return rc;
     const double narrow = deal(p, 1, pairs).time, wide = p.gated ? narrow : deal(p, 2, pairs).time;
-    *us = 6.0 + (narrow < wide ? narrow : wide);  // launch, set-up and the last epilogue
+    *us = (p.gated ? 7.5 : 6.0) + (narrow < wide ? narrow : wide);  // launch, set-up and the last epilogue
     return CUDAIR_OK;
 }
 

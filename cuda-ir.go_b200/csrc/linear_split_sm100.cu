@@ -31,6 +31,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "cudair_internal.h"
@@ -62,6 +63,7 @@ struct JobArgs {
     int num_kb, parts;   // k-blocks of one contraction; contractions per accumulator
     int mt;              // rows of D per tile, a multiple of 16 (of 64 where A's rows run along memory)
     int m_tiles, first;  // row tiles; the job's first tile
+    int run, longer;     // k-blocks of a rank; the first `longer` ranks take one more
     int w_mn, x_mn;
     uint32_t idesc;
     int w_early;  // B is a weight that nothing still running writes
@@ -79,6 +81,23 @@ struct Args {
     unsigned int *status;
 };
 
+__device__ __forceinline__ uint32_t cluster_id() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%clusterid.x;" : "=r"(r));
+    return r;
+}
+// All threads of the cluster; orders no memory accesses.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_shared_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -160,6 +179,104 @@ __device__ __forceinline__ void add4(uint4 r, bool f32, bool bf16, float (&v)[4]
 // allocates tensor memory; two of these do share an SM).
 __global__ void __launch_bounds__(threads(8), 2) occupancy_kernel() {}
 
+// The sums and the epilogue.  Rank r of SPLIT takes rows r, r + SPLIT, ... of the
+// tile; a warp takes whole rows, four columns a lane (`mine`: where the
+// lane's columns of this CTA's parts start).  An element's parts are added from
+// its own rank's on, round the ranks: a fixed order.  What bounds it is the
+// network between SMs, about 15 bytes a clock for each (64 rows of two ranks took
+// 5800 clocks when the own rank's part went through it too).
+template <bool GATED, int SPLIT, int EPI_WARPS>
+__device__ __forceinline__ void join(const Args &p, const JobArgs &job, uint32_t mine, int rank, int m0, int n0,
+                                     int rows) {
+    constexpr int W_TILES = GATED ? 2 : 1;
+    constexpr int WARPS = threads(EPI_WARPS) / 32;
+    constexpr int LOADS = SPLIT * W_TILES;  // per row
+    // Rows that are worked on together, as registers allow.
+    constexpr int BATCH = EPI_WARPS > 4 ? (LOADS >= 8 ? 1 : 2) : LOADS >= 16 ? 1 : LOADS >= 4 ? 2 : 4;
+    const uint32_t warp = warp_id();
+    const int mt = job.mt, col = n0 + static_cast<int>(lane_id()) * 4;
+    if (col >= job.N) return;
+    const bool bf16 = p.bf16 != 0;
+    float bias[4] = {};
+    if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + j < job.N)
+                bias[j] = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[col + j], bf16)
+                                   : static_cast<const float *>(p.bias)[col + j];
+    }
+    uint32_t from[SPLIT];
+#pragma unroll
+    for (int r = 1; r < SPLIT; ++r) from[r] = mapa_shared(mine, static_cast<uint32_t>((rank + r) % SPLIT));
+    const int own = (rows - rank + SPLIT - 1) / SPLIT;  // rows of this rank
+    for (int k0 = static_cast<int>(warp) * BATCH; k0 < own; k0 += WARPS * BATCH) {
+        // Row b of the batch is there.  (Without it, nothing is loaded: no read
+        // of another CTA's memory may be left that nothing waits for.)
+        auto there = [&](int b) { return k0 + b < own; };
+        auto row = [&](int b) { return rank + (k0 + b) * SPLIT; };
+        float v[W_TILES][BATCH][4] = {};
+        uint4 res[BATCH] = {};
+        {
+            float4 t[W_TILES][BATCH][SPLIT];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (!there(b)) break;
+#pragma unroll
+                for (int i = 0; i < W_TILES; ++i) {
+                    const uint32_t at = static_cast<uint32_t>(i * mt + row(b)) * (NT * 4);
+#pragma unroll
+                    for (int r = 1; r < SPLIT; ++r) t[i][b][r] = ld_cluster_f4(from[r] + at);
+                    t[i][b][0] = ld_shared_f4(mine + at);
+                }
+                if (p.residual.p) res[b] = fetch4(p.residual, m0 + row(b), col, job.N);
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (!there(b)) break;
+#pragma unroll
+                for (int i = 0; i < W_TILES; ++i)
+#pragma unroll
+                    for (int r = 0; r < SPLIT; ++r) {
+                        v[i][b][0] += t[i][b][r].x;
+                        v[i][b][1] += t[i][b][r].y;
+                        v[i][b][2] += t[i][b][r].z;
+                        v[i][b][3] += t[i][b][r].w;
+                    }
+            }
+        }
+        if (!GATED) {
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[0][b][j] += bias[j];
+        }
+        if (p.z[0].p) {
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (there(b)) {
+#pragma unroll
+                    for (int i = 0; i < W_TILES; ++i) store4(p.z[i], m0 + row(b), col, job.N, bf16, v[i][b]);
+                }
+        }
+        if (GATED || p.act != CUDAIR_ACT_NONE)
+            with_act(p.act, [&](auto tag) {
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[0][b][j] = act_value<decltype(tag)::value>(v[0][b][j]) *
+                                     (GATED ? v[W_TILES - 1][b][j] : 1.0f);
+            });
+        if (p.residual.p) {
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) add4(res[b], p.residual.f32, bf16, v[0][b]);
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+            if (there(b)) store4(job.d, m0 + row(b), col, job.N, bf16, v[0][b]);
+    }
+}
+
 template <bool GATED, int EPI_WARPS>
 __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     product_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args p) {
@@ -182,21 +299,33 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     float *part = reinterpret_cast<float *>(smem);  // the ring's memory, once the MMAs are done: [acc][m][n]
 
     const uint32_t warp = warp_id(), lane = lane_id();
-    const int rank = static_cast<int>(blockIdx.x % p.split);
-    int tile = static_cast<int>(blockIdx.x / p.split);
-    int ji = 0;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (threadIdx.x == 64) grid_launch_dependents();  // cudair_set_gemm_pdl
+
+    const int rank = static_cast<int>(cluster_ctarank());
+    int tile = static_cast<int>(cluster_id()), ji = 0;
     if (p.jobs > 1 && tile >= p.job[1].first) ji = p.jobs > 2 && tile >= p.job[2].first ? 2 : 1;
     const JobArgs job = ji == 0 ? p.job[0] : ji == 1 ? p.job[1] : p.job[2];  // fixed places: in registers
     tile -= job.first;
     const int mt = job.mt;
-    const int m0 = tile % job.m_tiles * mt, n0 = tile / job.m_tiles * NT;
+    int m0 = 0, n0 = tile * NT;
+    if (job.m_tiles > 1) {
+        const unsigned n = static_cast<unsigned>(tile) / static_cast<unsigned>(job.m_tiles);
+        m0 = (tile - static_cast<int>(n) * job.m_tiles) * mt;
+        n0 = static_cast<int>(n) * NT;
+    }
     const int rows = min(mt, job.M - m0);
-    const int total_kb = job.num_kb * job.parts;
-    const int kb0 = static_cast<int>(static_cast<long long>(total_kb) * rank / p.split);
-    const int kb1 = static_cast<int>(static_cast<long long>(total_kb) * (rank + 1) / p.split);
-
-    if (threadIdx.x == 64) grid_launch_dependents();  // cudair_set_gemm_pdl
-
+    const int kb0 = rank * job.run + min(rank, job.longer);
+    const int kb1 = kb0 + job.run + (rank < job.longer ? 1 : 0);
     const int head = min(kb1 - kb0, STAGES);
     const int part_kb = job.num_kb, w_mn = job.w_mn, x_mn = job.x_mn;
     const CUtensorMap *map_w = &maps.w[ji][0], *map_x = &maps.x[ji][0];
@@ -229,18 +358,10 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
         }
     };
 
-    // The producer thread sets up its barriers and requests the first
-    // ring-full at once: the rest of the set-up runs under the copies.  Its weights may be
-    // requested before the preceding kernel ends (launch mode 2).
+    // The producer thread, which set up the barriers, requests the first
+    // ring-full at once: the rest of the set-up runs under the copies.  Its
+    // weights may be requested before the preceding kernel ends (launch mode 2).
     if (threadIdx.x == 0) {
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
-        }
-        mbar_init(acc_full, 1);
-        mbar_init(drain, 1);
-        *abort_flag = 0;
-        fence_mbar_init();
         if (!job.w_early) grid_dependency_wait();
         for (int i = 0; i < head; ++i) {
             load_w(kb0 + i, i);
@@ -367,94 +488,24 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
         cluster_sync();
     else
         __syncthreads();
-
-    // ---------------- the sums and the epilogue ----------------
-    // Rank r takes rows r, r + split, ...; a warp takes whole rows of the tile,
-    // four columns a lane.
-    grid_dependency_wait();
-    const int col = n0 + static_cast<int>(lane) * 4;
-    if (col < job.N) {
-        const bool bf16 = p.bf16 != 0;
-        float bias[4] = {};
-        if (p.bias) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + j < job.N)
-                    bias[j] = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[col + j], bf16)
-                                       : static_cast<const float *>(p.bias)[col + j];
-        }
-        const uint32_t base = smem_u32(part) + lane * 16u;
-        constexpr int BATCH = GATED ? 1 : 2;  // rows whose parts are requested together
-        constexpr int WARPS = threads(EPI_WARPS) / 32;
-        const int own = (rows - rank + p.split - 1) / p.split;  // rows of this rank
-        for (int k0 = static_cast<int>(warp) * BATCH; k0 < own; k0 += WARPS * BATCH) {
-            float4 t[BATCH * W_TILES][MAX_SPLIT];
-            uint4 res[BATCH];
-            if (p.residual.p) {
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b)
-                    res[b] = fetch4(p.residual, m0 + rank + min(k0 + b, own - 1) * p.split, col, job.N);
-            }
-#pragma unroll
-            for (int r = 0; r < MAX_SPLIT; ++r)
-                if (r < p.split) {
-                    const uint32_t from = mapa_shared(base, r);
-#pragma unroll
-                    for (int b = 0; b < BATCH; ++b)
-#pragma unroll
-                        for (int i = 0; i < W_TILES; ++i) {
-                            const int c = rank + min(k0 + b, own - 1) * p.split;
-                            t[b * W_TILES + i][r] = ld_cluster_f4(from + (i * mt + c) * (NT * 4));
-                        }
-                }
-#pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                if (k0 + b >= own) break;
-                const int c = rank + (k0 + b) * p.split;
-                float v[W_TILES][4] = {};
-#pragma unroll
-                for (int r = 0; r < MAX_SPLIT; ++r)
-                    if (r < p.split) {
-#pragma unroll
-                        for (int i = 0; i < W_TILES; ++i) {
-                            v[i][0] += t[b * W_TILES + i][r].x;
-                            v[i][1] += t[b * W_TILES + i][r].y;
-                            v[i][2] += t[b * W_TILES + i][r].z;
-                            v[i][3] += t[b * W_TILES + i][r].w;
-                        }
-                    }
-                const long long row = m0 + c;
-                float out[4];
-                if (GATED) {
-                    if (p.z[0].p) {
-                        store4(p.z[0], row, col, job.N, bf16, v[0]);
-                        store4(p.z[1], row, col, job.N, bf16, v[W_TILES - 1]);
-                    }
-                    with_act(p.act, [&](auto tag) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            out[j] = act_value<decltype(tag)::value>(v[0][j]) * v[W_TILES - 1][j];
-                    });
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[0][j] += bias[j];
-                    if (p.z[0].p) store4(p.z[0], row, col, job.N, bf16, v[0]);
-                    with_act(p.act, [&](auto tag) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) out[j] = act_value<decltype(tag)::value>(v[0][j]);
-                    });
-                    if (p.residual.p) add4(res[b], p.residual.f32, bf16, out);
-                }
-                store4(job.d, row, col, job.N, bf16, out);
-            }
-        }
-    }
-    __syncwarp();
-    if (p.split > 1) cluster_sync();  // no rank leaves while its parts are being read
     if (warp == 1) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, p.tmem_cols);
     }
+
+    grid_dependency_wait();
+    const uint32_t mine = smem_u32(part) + lane * 16u;
+    switch (p.split) {
+        case 1: join<GATED, 1, EPI_WARPS>(p, job, mine, rank, m0, n0, rows); break;
+        case 2: join<GATED, 2, EPI_WARPS>(p, job, mine, rank, m0, n0, rows); break;
+        case 4: join<GATED, 4, EPI_WARPS>(p, job, mine, rank, m0, n0, rows); break;
+        default: join<GATED, 8, EPI_WARPS>(p, job, mine, rank, m0, n0, rows); break;
+    }
+    // No rank leaves while its parts are being read.  Relaxed: the reads are
+    // done, and the stores need no waiting for (a releasing barrier waits for
+    // them: 1.2 us).
+    __syncwarp();
+    if (p.split > 1) cluster_sync_relaxed();
 }
 
 // ---- host side -----------------------------------------------------------------------
@@ -524,84 +575,96 @@ int prepare_device(const Device **out) {
     return CUDAIR_OK;
 }
 
+// One way to cut a call.
+struct Cut {
+    int64_t tiles = 0, kb = 0;  // kb: k-blocks of the longest contraction
+    int w_tiles = 1, mt = 0, rows = 0, split = 1;
+    int two = 0;  // 1: the ring of two CTAs per SM
+    double weight_bytes = 0.0;
+};
+
+// How long the kernel takes for one way to cut a call, in microseconds.  Fitted
+// to 1800 timings of 82 shapes on B200 (1 to 1024 rows, 128 to 128256 columns,
+// 64 to 14336 deep; tiles of 16 to 128 rows, split 1 to 8; 9 % rms).  What it
+// says of the kernel:
+//   * launch, set-up and the end are 3.8 us, 0.5 us more for each CTA per SM, and
+//     0.65 us where some SMs get a second one; a further wave costs 2 us;
+//   * a CTA's k-blocks follow one another in 0.32 us at best, at 89 GB/s into an
+//     SM, and together no faster than HBM gives the weights: 5.9 TB/s to 112
+//     CTAs, 6.4 to 224 (16 x 14336 x 4096: 24.1 and 23.1 us);
+//   * a row of parts costs 13.6 ns on its way through shared memory, and 1.6 ns
+//     more through the network between SMs.
+double split_time(const Cut &c, const int (&clusters)[2][MAX_SPLIT + 1]) {
+    const double sms = clusters[0][1];
+    const double ctas = static_cast<double>(c.tiles) * c.split;
+    const double places = static_cast<double>(clusters[c.two][c.split]) * c.split;
+    const double waves = std::ceil(ctas / places), per_sm = std::max(1.0, std::min(ctas, places) / sms);
+    const double run = std::ceil(static_cast<double>(c.kb) / c.split);
+    const double stage = static_cast<double>(c.w_tiles) * W_TILE + c.mt * BK * 2;
+    const double block = std::max(std::max(0.32, stage * per_sm / 89e3), 0.124 * c.w_tiles * c.mt / 128 * per_sm);
+    const double hbm = 5.4e6 + 0.66e6 * std::min(ctas, places) / sms;  // bytes a microsecond
+    const double stream = std::max(waves * run * block, c.weight_bytes / hbm);
+    const double rows = static_cast<double>(c.rows) * c.w_tiles;
+    const double joins = (0.0016 * (c.split - 1) / c.split + 0.0136) * rows * std::max(1.0, 0.36 * per_sm) * waves;
+    return 3.8 + 0.49 * ctas / sms + (ctas > static_cast<double>(clusters[0][c.split]) * c.split ? 0.65 : 0.0) +
+           2.0 * (waves - 1.0) + stream + joins;
+}
+
 }  // namespace
 }  // namespace split
 
-// When the split kernel runs, and how it is cut.  A cut is good when all its
-// CTAs run at once: every further wave costs 4 to 5 us of set-up and join
-// (16 x 14336 x 4096, 112 tiles: split in 2, 224 CTAs on 296 places 23.6 us;
-// in 4, 448 CTAs, 28.2 us; in 8, 35.6 us).  So:
-//   tile rows  M rounded up to 16 up to M = 128, else 128; 64 above M = 64 where
-//              that still splits in four or more (256 x 1024 x 1024: 64 rows
-//              and split 4 7.6 us, 128 rows and split 6 8.7 us).
-//   split      the largest with one CTA per SM (512 x 512 x 512, 32 tiles: 4
-//              6.6 us, 8 with two CTAs per SM 9.5 us).  Where that is 2 or less and
-//              leaves a CTA 24 k-blocks or more, the largest with two per SM
-//              (1 x 14336 x 4096: 27.0 us for 1, 24.4 us for 2; weight gradient
-//              1024 x 1024 over 8192: 32.4 us for 2, 25.3 us for 4).
-//   ring       that of two CTAs per SM (a shorter first ring-full starts
-//              sooner: 1 x 256 x 8192 9.6 against 10.4 us), but a whole SM's where
-//              half of one holds three stages or fewer (128 x 4096 x 4096: 14.4 against
-//              15.5 us).
-// Against the pair kernel: up to M = 128 the split kernel, unless its tiles
-// exceed one wave above M = 96 (128 x 32768 x 2048: 36.6 against 32.6 us);
-// above, where the tiles leave room to split at all (1024 x 1024 x 4096 18.0
-// against 26.0 us; 1024 x 4096 x 4096, 256 tiles, 44.7 against 28.6 us).
-// Several jobs (the gradients of a call) share one grid; they go to the pair
-// kernel when one of them would alone.
+// The best way to cut a call: tiles of 16 to 128 rows, split 1, 2, 4 or 8, a
+// ring for one or two CTAs per SM.  Several jobs share one grid and the split.
+// Of two cuts that take the same, the ring of two CTAs per SM (a shorter first
+// ring-full starts sooner: 1 x 256 x 8192 9.6 against 10.4 us), but a whole SM's
+// where half of one holds three stages or fewer (128 x 4096 x 4096: 13.1 against 14.3 us).
 int split_plan(const Product &p, SplitPlan *plan) {
     using namespace split;
     const Device *dev = nullptr;
     const int rc = prepare_device(&dev);
     if (rc != CUDAIR_OK) return rc;
-    const int w_tiles = p.tiles_of_b();
-    // The largest split whose clusters all fit, with one or two CTAs per SM (0: none).
-    auto fits = [&](int64_t tiles, int64_t kb, int two) {
-        for (int s = static_cast<int>(std::min<int64_t>(MAX_SPLIT, std::max<int64_t>(kb, 1))); s > 0; --s)
-            if (tiles <= dev->clusters[two][s]) return s;
-        return 0;
-    };
-    plan->split = 0;
-    int64_t total = 0, most_kb = 0;
-    int most_mt = 0;
-    for (int i = 0; i < p.jobs; ++i) {
-        const Job &j = p.job[i];
-        const int64_t n_tiles = (j.N + NT - 1) / NT, kb = (j.K + BK - 1) / BK * j.parts;
-        auto tiles = [&](int mt) { return (j.M + mt - 1) / mt * n_tiles; };
-        const int unit = j.a[0].mn ? 64 : 16;
-        int mt = static_cast<int>(std::min<int64_t>(128, (j.M + unit - 1) / unit * unit));
-        const int one = fits(tiles(mt), kb, 0);
-        if (j.M > 128 ? one < 2 : j.M > 96 && one < 1) return CUDAIR_OK;
-        if (mt > 64 && p.jobs == 1 && fits(tiles(64), kb, 0) >= 4) mt = 64;
-        plan->mt[i] = mt;
-        most_mt = std::max(most_mt, mt);
-        most_kb = std::max(most_kb, kb);
-        total += tiles(mt);
+    plan->time = 1e30;
+    static constexpr int kRows[] = {16, 32, 48, 64, 96, 128};
+    for (const int want : kRows) {
+        Cut c;
+        c.w_tiles = p.tiles_of_b();
+        int mt[kMaxJobs] = {};
+        bool whole = true, fits = true;  // whole: no job has more rows than this
+        for (int i = 0; i < p.jobs; ++i) {
+            const Job &j = p.job[i];
+            // 64 rows at a time where A's rows run along memory.
+            const int unit = j.a[0].mn ? 64 : 16;
+            if (want % unit) fits = false;
+            mt[i] = static_cast<int>(std::min<int64_t>(want, (j.M + unit - 1) / unit * unit));
+            whole = whole && j.M <= want;
+            c.tiles += (j.M + mt[i] - 1) / mt[i] * ((j.N + NT - 1) / NT);
+            c.kb = std::max<int64_t>(c.kb, (j.K + BK - 1) / BK * j.parts);
+            c.mt = std::max(c.mt, mt[i]);
+            c.rows = std::max(c.rows, static_cast<int>(std::min<int64_t>(mt[i], j.M)));
+            c.weight_bytes += static_cast<double>(j.N) * static_cast<double>(j.K) * j.parts * c.w_tiles * 2.0;
+        }
+        if (!fits) continue;
+        const bool deep = c.w_tiles * static_cast<int>(W_TILE) + c.mt * BK * 2 > 28 * 1024;
+        for (int k = 0; k < 2; ++k) {
+            c.two = deep ? k : 1 - k;
+            const int stages = std::min(
+                MAX_STAGES, static_cast<int>((kBudget[c.two] - fixed_bytes()) / ring_bytes(c.w_tiles, c.mt, 1)));
+            // The parts take the ring's place.
+            if (ring_bytes(c.w_tiles, c.mt, stages) < static_cast<size_t>(c.w_tiles) * c.mt * NT * 4) continue;
+            for (c.split = 1; c.split <= MAX_SPLIT; c.split *= 2) {
+                if (c.split > std::max<int64_t>(c.kb, 1) || c.tiles * c.split > INT32_MAX) break;
+                const double t = split_time(c, dev->clusters);
+                if (t < plan->time) {
+                    plan->time = t;
+                    plan->split = c.split;
+                    plan->stages = stages;
+                    for (int i = 0; i < p.jobs; ++i) plan->mt[i] = mt[i];
+                }
+            }
+        }
+        if (whole) break;
     }
-    const int one = fits(total, most_kb, 0);
-    // A stage of which fewer than four fit half an SM.
-    const bool deep = w_tiles * static_cast<int>(W_TILE) + most_mt * BK * 2 > 28 * 1024;
-    const bool can_share = !(w_tiles == 2 && most_mt > 64);
-    int split = std::max(one, 1), two = deep ? 0 : 1;
-    // Where even whole tiles exceed one wave (wide N), two CTAs per SM overlap
-    // one's join with the other's stream.
-    if (can_share && (one == 0 || (one <= 2 && most_kb >= 24 * split))) {
-        split = std::max(fits(total, most_kb, 1), 1);
-        two = 1;
-    }
-    if (total * split > INT32_MAX)
-        return set_error(CUDAIR_ERR_INVALID, "cudair: linear: %lld tiles are too many", (long long)total);
-    plan->split = split;
-    // Launch, set-up and join, then a CTA's k-blocks at the pace that its share
-    // of an SM and of HBM allows (tiles of 128 rows: 16 k-blocks a CTA with 128 CTAs 13.7
-    // us, with 256 CTAs 18.9 us).
-    const double ctas = static_cast<double>(total * split), places = dev->clusters[two][split] * split;
-    const double per_sm = std::min(ctas, places) / dev->clusters[0][1];
-    plan->time = 5.5 + static_cast<double>((most_kb + split - 1) / split) * (0.3 + 0.29 * per_sm) *
-                           std::max(1.0, ctas / places);
-    plan->stages =
-        std::min(MAX_STAGES, static_cast<int>((kBudget[two] - fixed_bytes()) / ring_bytes(w_tiles, most_mt, 1)));
-    return CUDAIR_OK;
+    return plan->time < 1e30 ? CUDAIR_OK : set_error(CUDAIR_ERR_INVALID, "cudair: linear: too many tiles");
 }
 
 int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *status, cudaStream_t stream) {
@@ -620,6 +683,8 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
         o.mt = plan.mt[i];
         o.m_tiles = static_cast<int>((j.M + o.mt - 1) / o.mt);
         o.first = tiles;
+        o.run = o.num_kb * o.parts / plan.split;
+        o.longer = o.num_kb * o.parts % plan.split;
         tiles += o.m_tiles * static_cast<int>((j.N + NT - 1) / NT);
         most_mt = std::max(most_mt, o.mt);
         o.w_mn = j.b[0].mn;
@@ -651,19 +716,26 @@ int product_split_launch(const Product &p, const SplitPlan &plan, unsigned int *
     const bool many = most_mt > 32;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(plan.split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    unsigned attrs = 0;
+    if (plan.split > 1) {
+        attr[attrs].id = cudaLaunchAttributeClusterDimension;
+        attr[attrs].val.clusterDim.x = static_cast<unsigned>(plan.split);
+        attr[attrs].val.clusterDim.y = 1;
+        attr[attrs].val.clusterDim.z = 1;
+        ++attrs;
+    }
+    if (p.pdl()) {
+        attr[attrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[attrs].val.programmaticStreamSerializationAllowed = 1;
+        ++attrs;
+    }
     cfg.gridDim = dim3(static_cast<unsigned>(tiles) * plan.split, 1, 1);
     cfg.blockDim = dim3(static_cast<unsigned>(threads(many ? 8 : 4)), 1, 1);
     cfg.dynamicSmemBytes =
         std::max(fixed_bytes() + ring_bytes(w_tiles, most_mt, plan.stages), smem_floor(args.tmem_cols));
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = p.pdl() ? 2 : 1;
+    cfg.numAttrs = attrs;
     const cudaError_t e = p.gated ? (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<true, 8>, maps, args)
                                           : cudaLaunchKernelEx(&cfg, product_split_kernel<true, 4>, maps, args))
                                   : (many ? cudaLaunchKernelEx(&cfg, product_split_kernel<false, 8>, maps, args)
