@@ -293,34 +293,5 @@ __device__ __forceinline__ void add_row32(const Row32 &r, bool f32, bool bf16, f
     }
 }
 
-// Adds 32 values that every row shares, from a 16-byte aligned vector.
-__device__ __forceinline__ void add_row32_uniform(const void *p, bool is16, bool bf16, int col, float (&v)[32]) {
-    if (is16) {
-        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + col);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint4 w = q[j];
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float lo, hi;
-                unpack16(u[k], bf16, lo, hi);
-                v[8 * j + 2 * k] += lo;
-                v[8 * j + 2 * k + 1] += hi;
-            }
-        }
-    } else {
-        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p) + col);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float4 f = q[j];
-            v[4 * j] += f.x;
-            v[4 * j + 1] += f.y;
-            v[4 * j + 2] += f.z;
-            v[4 * j + 3] += f.w;
-        }
-    }
-}
-
 }  // namespace ffn
 }  // namespace cudair

@@ -55,7 +55,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int PM = 256;  // rows per pair tile, 128 per CTA
 constexpr uint32_t A_STAGE = 128 * BK * 2;
-constexpr uint32_t BAR_BYTES = 256;
+constexpr uint32_t BAR_BYTES = 256 + 512;  // barriers, and the jobs' arguments
 constexpr int GROUP_M = 8;  // row-blocks visited together (A and B panels shared in L2)
 
 // A tile takes NB accumulator blocks of BN columns (the MMA's N).  NB = 1: two
@@ -72,7 +72,7 @@ struct PairCfg {
     static constexpr int STAGES = static_cast<int>((227 * 1024 - 1024 - BAR_BYTES) / STAGE);
     static constexpr size_t SMEM = 1024 + STAGES * STAGE + BAR_BYTES;
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
-    static_assert(2 * STAGES * 8 + 5 * 8 + 8 <= BAR_BYTES, "barrier area");
+    static_assert(2 * STAGES * 8 + 5 * 8 + 8 <= 256, "barrier area");
 };
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -80,13 +80,25 @@ struct Maps {
     CUtensorMap a[kMaxJobs][2], b[kMaxJobs][2];
 };
 
+// Division by a fixed d of n < 2^31: (n mul) >> (31 + l) with l = ceil(log2 d)
+// and mul = ceil(2^(31 + l) / d), which is exact there.
+struct Div {
+    uint32_t mul, shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+    }
+};
+
 struct JobArgs {
+    Mat d;
     int M, N, num_m, num_n;
-    int num_kb, parts;  // k-blocks of one contraction; contractions per accumulator
+    int num_kb, all_kb;  // k-blocks of one contraction, and of all that an accumulator sums
     int a_mn, b_mn;
     uint32_t idesc;
-    Mat d;
+    int per_group;       // tiles of a group of GROUP_M row-blocks
+    Div group, last;     // by per_group; by the row-blocks of the last group
 };
+static_assert(sizeof(JobArgs) % 4 == 0, "copied by words");
 
 // The tiles of all jobs are numbered through, job after job.  Job 0 has the
 // longest ones: pair c takes its tiles c, c + C, ... (C pairs), so the first
@@ -96,19 +108,19 @@ struct JobArgs {
 struct PairArgs {
     JobArgs job[kMaxJobs];
     int first[kMaxJobs + 1];  // a job's first tile; the end
+    int own, more;            // tiles of job 0 of every pair; pairs that take one more
     int rounds;
     int act;
     Mat z[2], residual;
     const void *bias;
-    int bias16, bias_wide;  // bias_wide: 16-byte aligned
+    int bias16;
     unsigned int *status;
 };
 
 // The i-th tile of pair c of C, -1 after its last.
 __device__ __forceinline__ int tile_of(const PairArgs &p, int i, int c, int C) {
-    const int n0 = p.first[1], end = p.first[kMaxJobs];
-    const int more = n0 % C;  // pairs with one more tile of job 0
-    const int own = n0 / C + (c < more ? 1 : 0);
+    const int n0 = p.first[1], end = p.first[kMaxJobs], more = p.more;
+    const int own = p.own + (c < more ? 1 : 0);
     if (i < own) return i * C + c;
     const int j = i - own;
     int t = end;
@@ -125,13 +137,6 @@ struct Index {
 __device__ __forceinline__ int job_of(const PairArgs &p, int t) {
     return (t >= p.first[1] ? 1 : 0) + (t >= p.first[2] ? 1 : 0);
 }
-// A copy in registers, from fixed places in the arguments: an indexed place is
-// read through memory, again at every use between the kernel's asm statements
-// (gated 4096 x 14336 x 4096: 750 against 641 us).
-__device__ __forceinline__ JobArgs job_at(const PairArgs &p, int j) {
-    return j == 0 ? p.job[0] : j == 1 ? p.job[1] : p.job[2];
-}
-
 __device__ __forceinline__ void drain_wait(uint64_t *bar, uint32_t parity, unsigned int *status) {
     int never = 0;
     mbar_wait(bar, parity, &never, status, kSiteDrain);
@@ -139,15 +144,14 @@ __device__ __forceinline__ void drain_wait(uint64_t *bar, uint32_t parity, unsig
 
 // Tile index -> row-block and column-block: groups of GROUP_M row-blocks
 // visited column by column, every other group from the far end.
-__device__ __forceinline__ void tile_coords(int t, int num_m, int num_n, int &m_blk, int &n_blk) {
-    const int per_group = GROUP_M * num_n;
-    const int group = t / per_group;
+__device__ __forceinline__ void tile_coords(const JobArgs &job, int t, int &m_blk, int &n_blk) {
+    const int group = job.group(t);
     const int first_m = group * GROUP_M;
-    const int gsize = min(num_m - first_m, GROUP_M);
-    const int r = t - group * per_group;
-    m_blk = first_m + r % gsize;
-    n_blk = r / gsize;
-    if (group & 1) n_blk = num_n - 1 - n_blk;
+    const int r = t - group * job.per_group;
+    const int left = job.num_m - first_m;
+    n_blk = left >= GROUP_M ? r / GROUP_M : job.last(r);
+    m_blk = first_m + r - n_blk * (left >= GROUP_M ? GROUP_M : left);
+    if (group & 1) n_blk = job.num_n - 1 - n_blk;
 }
 
 __device__ __forceinline__ void load_acc(bool any, uint32_t taddr, float (&v)[32]) {
@@ -163,27 +167,41 @@ __device__ __forceinline__ void load_acc(bool any, uint32_t taddr, float (&v)[32
     }
 }
 
+// Arrives on an mbarrier of the cluster without ordering memory: what it hands
+// over is tensor memory whose loads have completed.  (A releasing arrival first waits
+// for the warp's stores to D: 3500 clocks a tile.)
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Columns of D that one epilogue warp takes of an accumulator block: two warps
 // share the block's 32 rows of a TMEM lane quarter.
 template <bool GATED>
 constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
 
 // One warp's 32 rows (one per lane) and kWarpCols columns from n0 on; t_row is
-// where they start in TMEM.  `next` holds the residual's first 32 columns,
-// requested before the accumulator was waited for; each further 32 are
-// requested while the ones before them are worked on.
+// where they start in TMEM.  `next` holds the residual's first 32 columns, and lane
+// l of `bias` the warp's columns l, l + 32, ...: both were requested before the
+// accumulator was waited for.  The residual's further columns are requested while the
+// ones before them are worked on.
 template <bool GATED, bool bf16>
 __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row, int n0, bool live,
-                                               bool any, Row32 &next) {
+                                               bool any, Row32 &next, const float (&bias)[kWarpCols<GATED> / 32], uint32_t acc_empty) {
 #pragma unroll 1
     for (int c = 0; c < kWarpCols<GATED>; c += 32) {
         const int col = n0 + c;
         if (col >= job.N) break;
-        float v[32];
+        float v[32], u[GATED ? 32 : 1];
         load_acc(any, t_row + c, v);
-        if (GATED) {
-            float u[32];
-            load_acc(any, t_row + BN / 2 + c, u);
+        if constexpr (GATED) load_acc(any, t_row + BN / 2 + c, u);
+        // The last columns are read: the block goes back to the MMA warp while
+        // they are worked on.
+        if (any && (c + 32 >= kWarpCols<GATED> || col + 32 >= job.N)) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane_id() == 0) mbar_arrive_cluster_relaxed(acc_empty);
+        }
+        if constexpr (GATED) {
             if (p.z[0].p && live) {
                 store_row32(p.z[0], row, col, job.N, bf16, v);
                 store_row32(p.z[1], row, col, job.N, bf16, u);
@@ -194,20 +212,12 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
             });
         } else {
             if (p.bias) {
-                // Every lane adds the same 32 values: whole blocks by uniform
-                // 16-byte loads, a last one that ends inside the 32 through a
-                // shuffle of lane l's column l.
-                if (p.bias_wide && col + 32 <= job.N) {
-                    add_row32_uniform(p.bias, p.bias16, bf16, col, v);
-                } else {
-                    float b = 0.0f;
-                    const int bc = col + static_cast<int>(lane_id());
-                    if (bc < job.N)
-                        b = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], bf16)
-                                     : static_cast<const float *>(p.bias)[bc];
+                float mine = bias[0];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, b, j);
-                }
+                for (int k = 1; k < kWarpCols<GATED> / 32; ++k)
+                    if (c == 32 * k) mine = bias[k];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, mine, j);
             }
             if (p.z[0].p && live) store_row32(p.z[0], row, col, job.N, bf16, v);
             if (p.act != CUDAIR_ACT_NONE)
@@ -246,6 +256,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *drain = acc_empty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    // The jobs' arguments: indexed here they are read from shared memory, where
+    // an indexed place in the arguments themselves is read through memory, again at
+    // every use between asm statements (gated 4096 x 14336 x 4096: 750 against 641 us).
+    JobArgs *jobs = reinterpret_cast<JobArgs *>(reinterpret_cast<uint8_t *>(bars) + 256);
+    static_assert(kMaxJobs * sizeof(JobArgs) <= BAR_BYTES - 256, "jobs area");
 
     const uint32_t warp = warp_id(), lane = lane_id();
     const uint32_t rank = cluster_ctarank();  // 0 = even CTA (issues the MMAs)
@@ -270,6 +285,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_alloc_pair(tmem_slot, TMEM_COLS);
         tmem_relinquish_pair();
     }
+    if (threadIdx.x < kMaxJobs * sizeof(JobArgs) / 4)
+        reinterpret_cast<uint32_t *>(jobs)[threadIdx.x] = reinterpret_cast<const uint32_t *>(p.job)[threadIdx.x];
+    __syncwarp();
     tc_fence_before_sync();
     cluster_sync();  // barriers of both CTAs initialised before any remote arrive
     tc_fence_after_sync();
@@ -292,9 +310,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             auto load_tile = [&](auto tag, int t) -> bool {
                 constexpr int J = decltype(tag)::value;
                 const JobArgs &job = p.job[J];
-                const int num_kb = job.num_kb * job.parts;
+                const int num_kb = job.all_kb;
                 int m_blk, n_blk;
-                tile_coords(t, job.num_m, job.num_n, m_blk, n_blk);
+                tile_coords(job, t, m_blk, n_blk);
                 const CUtensorMap *ma = &maps.a[J][0], *mb = &maps.b[J][GATED ? rank : 0];
                 // Rows and columns beyond the matrices arrive as zeros (the
                 // maps clip), so every stage carries the same bytes.
@@ -430,8 +448,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 return true;
             };
             for (int i = 0, t; ok && (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
-                const JobArgs job = job_at(p, job_of(p, t));
-                const int num_kb = job.num_kb * job.parts;
+                const JobArgs &job = jobs[job_of(p, t)];
+                const int num_kb = job.all_kb;
                 if (num_kb == 0) continue;  // an empty sum: the epilogue's alone
                 a_step = job.a_mn ? 2048u : 32u;
                 a_lbo = job.a_mn ? 64u * BK * 2 : 16u;
@@ -468,10 +486,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t acc = 0, acc_phase = 0;
         for (int i = 0, t; (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
             const int j = job_of(p, t);
-            const JobArgs job = job_at(p, j);
-            const int num_kb = job.num_kb * job.parts;
+            const JobArgs job = jobs[j];
+            const int num_kb = job.all_kb;
             int m_blk, n_blk;
-            tile_coords(t - p.first[j], job.num_m, job.num_n, m_blk, n_blk);
+            tile_coords(job, t - p.first[j], m_blk, n_blk);
             const int row0 = m_blk * PM + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
             const int row = row0 + static_cast<int>(lane);
             const int n0 = n_blk * TILE_N;
@@ -482,6 +500,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t bar = acc + h;  // NB = 2: block h's own barriers
                 const int col0 = n0 + h * BLOCK_N + side * kWarpCols<GATED>;
                 Row32 res;
+                float bias[kWarpCols<GATED> / 32] = {};
+                if (!GATED && p.bias) {
+#pragma unroll
+                    for (int k = 0; k < kWarpCols<GATED> / 32; ++k) {
+                        const int bc = col0 + 32 * k + static_cast<int>(lane);
+                        if (bc < job.N)
+                            bias[k] = p.bias16 ? from16(static_cast<const uint16_t *>(p.bias)[bc], BF16)
+                                               : static_cast<const float *>(p.bias)[bc];
+                    }
+                }
                 if (!GATED && p.residual.p && live && col0 < job.N)
                     fetch_row32(p.residual, row, col0, job.N, res);
                 if (num_kb > 0) {
@@ -493,12 +521,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                     __syncwarp();
                     tc_fence_after_sync();
                 }
+                const uint32_t mine_empty = mapa_shared(smem_u32(&acc_empty[bar]), 0);
                 const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + side * kWarpCols<GATED>;
-                if (row0 < job.M)  // the whole warp: TMEM loads are warp-wide
-                    epilogue_block<GATED, BF16>(p, job, t_row, row, col0, live, num_kb > 0, res);
-                tc_fence_before_sync();
+                if (row0 < job.M && col0 < job.N)  // the whole warp: TMEM loads are warp-wide
+                    epilogue_block<GATED, BF16>(p, job, t_row, row, col0, live, num_kb > 0, res, bias, mine_empty);
+                else if (num_kb > 0 && lane == 0)  // nothing of it lies in D
+                    mbar_arrive_cluster_relaxed(mine_empty);
                 __syncwarp();
-                if (num_kb > 0 && lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[bar]), 0));
             }
             if (aborted) break;
             if (num_kb > 0) {
@@ -534,6 +563,15 @@ int operand_map(CUtensorMap *out, const Operand &o, int64_t rows, int64_t depth,
 }
 
 namespace {
+
+Div divide_by(int d) {
+    Div v;
+    uint32_t l = 0;
+    while ((1ll << l) < d) ++l;
+    v.shift = 31 + l;
+    v.mul = static_cast<uint32_t>(((1ull << v.shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
+    return v;
+}
 
 std::mutex g_pair_mu;
 int g_pairs[64];  // CTA pairs resident at once, per device (0: not asked yet)
@@ -694,6 +732,9 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     const int tile_n = BN * nb / p.tiles_of_b();
     for (int i = 0; i <= kMaxJobs; ++i) args.first[i] = static_cast<int>(d.first[i]);
     args.rounds = static_cast<int>(d.rounds);
+    const int C = args.first[kMaxJobs] < pairs ? args.first[kMaxJobs] : pairs;
+    args.own = args.first[1] / C;
+    args.more = args.first[1] % C;
     for (int i = 0; i < p.jobs; ++i) {
         const Job &j = p.job[d.order[i]];
         JobArgs &o = args.job[i];
@@ -702,7 +743,10 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
         o.num_m = static_cast<int>((j.M + PM - 1) / PM);
         o.num_n = static_cast<int>((j.N + tile_n - 1) / tile_n);
         o.num_kb = static_cast<int>((j.K + BK - 1) / BK);
-        o.parts = j.parts;
+        o.all_kb = o.num_kb * j.parts;
+        o.per_group = GROUP_M * o.num_n;
+        o.group = divide_by(o.per_group);
+        o.last = divide_by((o.num_m - 1) % GROUP_M + 1);
         o.a_mn = j.a[0].mn;
         o.b_mn = j.b[0].mn;
         o.idesc = idesc_f16_f32(PM, BN, j.a[0].mn, j.b[0].mn, p.bf16);
@@ -718,7 +762,6 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     args.residual = mat_of(p.residual);
     args.bias = p.bias;
     args.bias16 = p.bias16;
-    args.bias_wide = (reinterpret_cast<uintptr_t>(p.bias) & 15u) == 0;
     args.status = status;
     const bool pdl = p.pdl();
     const cudaError_t e = p.gated ? launch_pair<true, 1>(maps, args, pairs, p.bf16, pdl, stream)
