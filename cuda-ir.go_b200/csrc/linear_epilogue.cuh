@@ -68,24 +68,91 @@ __device__ __forceinline__ void normal_integral(float z, float &P, float &E) {
     P = z < 0.0f ? h : 1.0f - h;
 }
 
+// ---- two values at a time --------------------------------------------------------
+//
+// fma, mul and add on pairs of fp32 values are one instruction each on sm_100,
+// rounded as the single ones.  An epilogue's instructions are half of its time, so
+// its activations work on pairs (a chunk of 32 columns with gelu: 20 instructions a
+// value one by one, 9 in pairs; what remains is the two hardware functions).
+
+struct Pair {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ Pair pair(float both) { return pair(both, both); }
+__device__ __forceinline__ void unpair(Pair p, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair exp2_fast2(Pair p) {
+    float a, b;
+    unpair(p, a, b);
+    return pair(exp2_fast(a), exp2_fast(b));
+}
+__device__ __forceinline__ Pair rcp_fast2(Pair p) {
+    float a, b;
+    unpair(p, a, b);
+    return pair(rcp_fast(a), rcp_fast(b));
+}
+// max(z, 0), a NaN kept.
+__device__ __forceinline__ float relu(float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(z));
+    return r;
+}
+
+// act(a), act(b) in place.  gelu: z P(z) = max(z, 0) - |z| T, T the upper tail at
+// |z| that normal_integral computes; |z| is held below 1e18, where T is 0, so
+// that an infinite z gives no 0 times infinity.
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-    if (ACT == CUDAIR_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (ACT == CUDAIR_ACT_SILU) return z * sigmoid(z);
-    if (ACT == CUDAIR_ACT_GELU) {
-        float P, E;
-        normal_integral(z, P, E);
-        return z * P;
+__device__ __forceinline__ void act_pair(float &a, float &b) {
+    if (ACT == CUDAIR_ACT_RELU) {
+        a = relu(a);
+        b = relu(b);
+    } else if (ACT == CUDAIR_ACT_SILU) {
+        const Pair z = pair(a, b);
+        const Pair e = exp2_fast2(mul2(z, pair(-kLog2E)));
+        unpair(mul2(z, rcp_fast2(add2(e, pair(1.0f)))), a, b);
+    } else if (ACT == CUDAIR_ACT_GELU_TANH) {
+        const Pair z = pair(a, b);
+        const Pair y = fma2(mul2(z, z), pair(-kLog2E * kGeluC * kGeluB), pair(-kLog2E * kGeluC));
+        unpair(mul2(z, rcp_fast2(add2(exp2_fast2(mul2(z, y)), pair(1.0f)))), a, b);
+    } else if (ACT == CUDAIR_ACT_GELU) {
+        const Pair u = pair(fminf(fabsf(a), 1e18f), fminf(fabsf(b), 1e18f));
+        const Pair E = exp2_fast2(mul2(mul2(u, pair(-0.5f * kLog2E)), u));
+        const Pair t = rcp_fast2(fma2(u, pair(0.3275911f * 0.7071067811865476f), pair(1.0f)));
+        Pair h = fma2(t, pair(0.5f * 1.061405429f), pair(0.5f * -1.453152027f));
+        h = fma2(t, h, pair(0.5f * 1.421413741f));
+        h = fma2(t, h, pair(0.5f * -0.284496736f));
+        h = fma2(t, h, pair(0.5f * 0.254829592f));
+        h = mul2(h, mul2(t, E));
+        unpair(fma2(mul2(u, pair(-1.0f)), h, pair(relu(a), relu(b))), a, b);
     }
-    if (ACT == CUDAIR_ACT_GELU_TANH) return z * gelu_tanh_sigmoid(z, z * z);
-    return z;
 }
 
 // The value and the derivative at z.
 template <int ACT>
 __device__ __forceinline__ void act_both(float z, float &value, float &grad) {
     if (ACT == CUDAIR_ACT_RELU) {
-        value = z < 0.0f ? 0.0f : z;
+        value = relu(z);
         grad = z <= 0.0f ? 0.0f : 1.0f;
     } else if (ACT == CUDAIR_ACT_SILU) {
         const float s = sigmoid(z);
@@ -287,8 +354,7 @@ __device__ __forceinline__ void add_row32(const Row32 &r, bool f32, bool bf16, f
         for (int j = 0; j < 16; ++j) {
             float lo, hi;
             unpack16(r.w[j], bf16, lo, hi);
-            v[2 * j] += lo;
-            v[2 * j + 1] += hi;
+            unpair(add2(pair(v[2 * j], v[2 * j + 1]), pair(lo, hi)), v[2 * j], v[2 * j + 1]);
         }
     }
 }

@@ -208,7 +208,10 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
             }
             with_act(p.act, [&](auto tag) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]) * u[j];
+                for (int j = 0; j < 32; j += 2) {
+                    act_pair<decltype(tag)::value>(v[j], v[j + 1]);
+                    unpair(mul2(pair(v[j], v[j + 1]), pair(u[j], u[j + 1])), v[j], v[j + 1]);
+                }
             });
         } else {
             if (p.bias) {
@@ -217,13 +220,16 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
                 for (int k = 1; k < kWarpCols<GATED> / 32; ++k)
                     if (c == 32 * k) mine = bias[k];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] += __shfl_sync(0xFFFFFFFFu, mine, j);
+                for (int j = 0; j < 32; j += 2)
+                    unpair(add2(pair(v[j], v[j + 1]),
+                               pair(__shfl_sync(0xFFFFFFFFu, mine, j), __shfl_sync(0xFFFFFFFFu, mine, j + 1))),
+                          v[j], v[j + 1]);
             }
             if (p.z[0].p && live) store_row32(p.z[0], row, col, job.N, bf16, v);
             if (p.act != CUDAIR_ACT_NONE)
                 with_act(p.act, [&](auto tag) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = act_value<decltype(tag)::value>(v[j]);
+                    for (int j = 0; j < 32; j += 2) act_pair<decltype(tag)::value>(v[j], v[j + 1]);
                 });
             if (p.residual.p && live) {
                 add_row32(next, p.residual.f32, bf16, v);

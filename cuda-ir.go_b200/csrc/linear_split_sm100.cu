@@ -263,9 +263,13 @@ __device__ __forceinline__ void join(const Args &p, const JobArgs &job, uint32_t
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[0][b][j] = act_value<decltype(tag)::value>(v[0][b][j]) *
-                                     (GATED ? v[W_TILES - 1][b][j] : 1.0f);
+                    for (int j = 0; j < 4; j += 2) {
+                        act_pair<decltype(tag)::value>(v[0][b][j], v[0][b][j + 1]);
+                        if (GATED) {
+                            v[0][b][j] *= v[W_TILES - 1][b][j];
+                            v[0][b][j + 1] *= v[W_TILES - 1][b][j + 1];
+                        }
+                    }
             });
         if (p.residual.p) {
 #pragma unroll
