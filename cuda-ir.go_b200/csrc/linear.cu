@@ -14,6 +14,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <initializer_list>
+
 #include "cudair_internal.h"
 #include "linear_epilogue.cuh"
 #include "linear_internal.h"
@@ -294,6 +296,24 @@ int check_sizes(const char *op, int64_t M, int64_t N, int64_t K) {
     return CUDAIR_OK;
 }
 
+// A contraction's length is bounded so that one tile's k-blocks take well under the
+// two seconds after which a device wait gives up.
+constexpr int64_t kMaxDepth = int64_t{1} << 26;
+int check_depth(const char *op, int64_t depth) {
+    if (depth > kMaxDepth)
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a contraction over %lld is too long (at most %lld)", op,
+                         (long long)depth, (long long)kMaxDepth);
+    return CUDAIR_OK;
+}
+
+// An output in the place of an input or of another output.
+int check_distinct(const char *op, const char *name, const void *out, std::initializer_list<const void *> others) {
+    for (const void *o : others)
+        if (out && out == o)
+            return set_error(CUDAIR_ERR_INVALID, "cudair: %s: %s lies over another matrix of the call", op, name);
+    return CUDAIR_OK;
+}
+
 int check_flags(const char *op, uint32_t flags, uint32_t known, uint32_t act) {
     if (flags & ~known) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: unknown flags 0x%x", op, flags & ~known);
     if (act > CUDAIR_ACT_SILU)
@@ -377,7 +397,8 @@ int product_launch(const Product &p, cudaStream_t stream) {
     CUDAIR_TRY(sm_count_current_device(&sms));
     Launch all;
     CUDAIR_TRY(plan_launch(p, sms, &all));
-    if (p.jobs > 1) {
+    constexpr double kTwoLaunches = 8.6;  // no two launches take less
+    if (p.jobs > 1 && all.time > kTwoLaunches) {
         // A call's gradients share one launch (4096 x 14336 x 4096: linear 752 ->
         // 711 us, gated 1402 -> 1335 us; 301 x 515 x 1029 26 -> 15 us), unless the
         // first, whose contraction may be the longest, has few tiles that the
@@ -425,6 +446,10 @@ CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     if (q->z) CUDAIR_TRY(check_mat(op, "z", q->z, q->ldz, q->N, 2));
     if (q->bias && (reinterpret_cast<uintptr_t>(q->bias) & (bias16 ? 1u : 3u)))
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: bias must be aligned to its elements", op);
+    CUDAIR_TRY(check_depth(op, q->K));
+    const void *a = q->K > 0 ? q->a : nullptr, *b = q->K > 0 ? q->b : nullptr;
+    CUDAIR_TRY(check_distinct(op, "d", q->d, {a, b, q->bias, q->z}));
+    CUDAIR_TRY(check_distinct(op, "z", q->z, {a, b, q->bias, q->residual}));
     if (q->residual == q->d && q->residual && q->ldres != q->ldd)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a residual in D's memory needs D's pitch", op);
     Product p;
@@ -465,6 +490,11 @@ CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
         CUDAIR_TRY(check_mat(op, "g", q->g, q->ldg, q->N, 2));
         CUDAIR_TRY(check_mat(op, "u", q->u, q->ldu, q->N, 2));
     }
+    CUDAIR_TRY(check_depth(op, q->K));
+    const void *x = q->K > 0 ? q->x : nullptr, *wg = q->K > 0 ? q->wg : nullptr, *wu = q->K > 0 ? q->wu : nullptr;
+    CUDAIR_TRY(check_distinct(op, "h", q->h, {x, wg, wu, q->g, q->u}));
+    CUDAIR_TRY(check_distinct(op, "g", q->g, {x, wg, wu, q->u}));
+    CUDAIR_TRY(check_distinct(op, "u", q->u, {x, wg, wu}));
     Product p;
     p.jobs = 1;
     p.gated = true;
@@ -523,6 +553,14 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
     }
     if (q->dbias && (reinterpret_cast<uintptr_t>(q->dbias) & 3u))
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dbias must be 4-byte aligned", op);
+    if (want_da) CUDAIR_TRY(check_depth(op, q->N));
+    if (want_db) CUDAIR_TRY(check_depth(op, q->M));
+    if (q->M > 0 && q->N > 0 && q->K > 0) {
+        CUDAIR_TRY(check_distinct(op, "dz", q->dz, {q->a, q->b, q->da, q->db, q->dbias}));
+        CUDAIR_TRY(check_distinct(op, "da", q->da, {q->a, q->b, q->dy, q->z, q->db, q->dbias}));
+        CUDAIR_TRY(check_distinct(op, "db", q->db, {q->a, q->b, q->dy, q->z, q->dbias}));
+        CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->a, q->b, q->dy, q->z}));
+    }
 
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
@@ -612,6 +650,15 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         CUDAIR_TRY(check_mat(op, "dwg", q->dwg, q->lddwg, wcols, dw_f32 ? 4 : 2));
         CUDAIR_TRY(check_mat(op, "dwu", q->dwu, q->lddwu, wcols, dw_f32 ? 4 : 2));
         if (q->M > 0) CUDAIR_TRY(check_mat(op, "x", q->x, q->ldx, q->K, 2));
+    }
+    if (want_dx) CUDAIR_TRY(check_depth(op, q->N));
+    if (want_dw) CUDAIR_TRY(check_depth(op, q->M));
+    if (q->M > 0 && q->N > 0 && q->K > 0) {
+        CUDAIR_TRY(check_distinct(op, "dg", q->dg, {q->x, q->wg, q->wu, q->dx, q->dwg, q->dwu}));
+        CUDAIR_TRY(check_distinct(op, "du", q->du, {q->x, q->wg, q->wu, q->dx, q->dwg, q->dwu}));
+        CUDAIR_TRY(check_distinct(op, "dx", q->dx, {q->x, q->wg, q->wu, q->dh, q->g, q->u, q->dwg, q->dwu}));
+        CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->x, q->wg, q->wu, q->dh, q->g, q->u, q->dwu}));
+        CUDAIR_TRY(check_distinct(op, "dwu", q->dwu, {q->x, q->wg, q->wu, q->dh, q->g, q->u}));
     }
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks

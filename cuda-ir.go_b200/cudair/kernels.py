@@ -149,7 +149,7 @@ def _current_stream(stream, device):
 
 def _dims(op, x, xname, w, wname, b_trans):
     """(M, N, K) of x (M x K) and a weight (K x N, or N x K with b_trans)."""
-    if x.dim() != 2 or w.dim() != 2:
+    if getattr(x, "ndim", 0) != 2 or getattr(w, "ndim", 0) != 2:
         raise CudairError(1, f"cudair: {op}: {xname} and {wname} must be matrices")
     return x.shape[0], w.shape[0 if b_trans else 1], x.shape[1]
 
@@ -183,7 +183,8 @@ def linear(a, b, d, bias=None, residual=None, z=None, act="none", b_trans=False,
     if z is not None:
         pz, ldz = _mat(op, "z", z, t16, M, N, dev)
     check(lib().cudair_linear(ctypes.byref(LinearArgs(
-        pa, pb, pbias, pres, pd, pz, M, N, K, lda, ldb, ldres, ldd, ldz, _act(op, act), flags)), _current_stream(stream, dev)))
+        pa, pb, pbias, pres, pd, pz, M, N, K, lda, ldb, ldres, ldd, ldz, _act(op, act), flags)),
+        _current_stream(stream, dev)))
 
 
 def linear_backward(dy, a, b, z=None, dz=None, da=None, db=None, dbias=None, act="none", b_trans=False,

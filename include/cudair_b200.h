@@ -366,9 +366,11 @@ enum {
  *   z          M x N of A's type: Z as the backward pass reads it.
  * Every matrix is row-major with a 16-byte aligned base and a pitch of
  * whole 16 bytes; pitches are in elements.  No other output may overlap an
- * input.  M or N of 0 is a no-op; K of 0 gives act(bias) + residual (A and B
- * are not read).  Needs no workspace, so calls may overlap on several
- * streams.  Runs on stream, asynchronously, and follows
+ * input or another output.  M or N of 0 is a no-op; K of 0 gives act(bias) +
+ * residual (A and B are not read); K is at most 2^26.  A row of A that holds a
+ * NaN or an infinity reaches its row of D only, a column of B its column.
+ * Needs no workspace, so calls may overlap on several streams and in several
+ * graphs.  Runs on stream, asynchronously, and follows
  * cudair_set_gemm_pdl.
  */
 typedef struct cudair_linear_args {
@@ -392,8 +394,11 @@ int cudair_linear(const cudair_linear_args *args, void *stream);
  * CUDAIR_ACT_NONE or dY is fp32, and must be NULL otherwise (dY serves); it
  * may be dY's or z's own memory (same pitch).  z is needed where act is not
  * CUDAIR_ACT_NONE.  da, db and dbias may be NULL, and what only they need (b,
- * a) too.  Outputs are written, not added to.  M of 0 gives dB = 0 and
- * dbias = 0, N of 0 gives dA = 0.  Layout rules as cudair_linear.
+ * a) too.  Outputs are written, not added to, and their sums do not depend on
+ * timing.  M of 0 gives dB = 0 and dbias = 0, N of 0 gives dA = 0; the lengths
+ * that are summed over (N for dA, M for dB) are at most 2^26.  Layout rules as
+ * cudair_linear.  Runs two or three kernels, the later ones launched while
+ * the ones before end, in every mode of cudair_set_gemm_pdl.
  */
 typedef struct cudair_linear_backward_args {
     const void *dy, *a, *b, *z;

@@ -11,28 +11,33 @@ P = 0x7F0000000000  # a 16-byte aligned address; never dereferenced on CPU
 BF16, B_T, D_F32, BIAS_16, DA_F32, DB_F32 = 0x1, 0x2, 0x10, 0x20, 0x40, 0x80
 
 
+def _at(i):
+    """The i-th of some separate arrays."""
+    return P + (i << 20)
+
+
 def _linear(**over):
-    a = dict(a=P, b=P, bias=None, residual=None, d=P, z=None, M=4, N=24, K=16, lda=16, ldb=24, ldres=0, ldd=24,
-             ldz=0, act=0, flags=0)
+    a = dict(a=_at(0), b=_at(1), bias=None, residual=None, d=_at(2), z=None, M=4, N=24, K=16, lda=16, ldb=24,
+             ldres=0, ldd=24, ldz=0, act=0, flags=0)
     return "cudair_linear", _lib.LinearArgs(**{**a, **over})
 
 
 def _gated(**over):
-    a = dict(x=P, wg=P, wu=P, h=P, g=None, u=None, M=4, N=24, K=16, ldx=16, ldwg=24, ldwu=24, ldh=24, ldg=0,
-             ldu=0, act=4, flags=0)
+    a = dict(x=_at(0), wg=_at(1), wu=_at(2), h=_at(3), g=None, u=None, M=4, N=24, K=16, ldx=16, ldwg=24, ldwu=24,
+             ldh=24, ldg=0, ldu=0, act=4, flags=0)
     return "cudair_gated", _lib.GatedArgs(**{**a, **over})
 
 
 def _linear_backward(**over):
-    a = dict(dy=P, a=P, b=P, z=P, dz=P + 4096, da=P, db=P, dbias=P, M=4, N=24, K=16, lddy=24, lda=16, ldb=24,
-             ldz=24, lddz=24, ldda=16, lddb=24, act=2, flags=0)
+    a = dict(dy=_at(0), a=_at(1), b=_at(2), z=_at(3), dz=_at(4), da=_at(5), db=_at(6), dbias=_at(7), M=4, N=24,
+             K=16, lddy=24, lda=16, ldb=24, ldz=24, lddz=24, ldda=16, lddb=24, act=2, flags=0)
     return "cudair_linear_backward", _lib.LinearBackwardArgs(**{**a, **over})
 
 
 def _gated_backward(**over):
-    a = dict(dh=P, x=P, wg=P, wu=P, g=P, u=P, dg=P + 4096, du=P + 8192, dx=P, dwg=P, dwu=P, M=4, N=24, K=16,
-             lddh=24, ldx=16, ldwg=24, ldwu=24, ldg=24, ldu=24, lddg=24, lddu=24, lddx=16, lddwg=24, lddwu=24,
-             act=4, flags=0)
+    a = dict(dh=_at(0), x=_at(1), wg=_at(2), wu=_at(3), g=_at(4), u=_at(5), dg=_at(6), du=_at(7), dx=_at(8),
+             dwg=_at(9), dwu=_at(10), M=4, N=24, K=16, lddh=24, ldx=16, ldwg=24, ldwu=24, ldg=24, ldu=24, lddg=24,
+             lddu=24, lddx=16, lddwg=24, lddwu=24, act=4, flags=0)
     return "cudair_gated_backward", _lib.GatedBackwardArgs(**{**a, **over})
 
 
@@ -53,7 +58,7 @@ def _gated_backward(**over):
     (_linear(ldd=25), "pitch 25 of d must be a multiple of 8"),
     (_linear(flags=D_F32, ldd=26), "pitch 26 of d must be a multiple of 4"),
     (_linear(residual=P, ldres=8), "pitch 8 of residual is below"),
-    (_linear(residual=P, ldres=32), "a residual in D's memory needs D's pitch"),
+    (_linear(residual=_at(2), ldres=32), "a residual in D's memory needs D's pitch"),
     (_linear(z=P + 1, ldz=24), "z must be 16-byte aligned"),
     (_linear(bias=P + 2), "bias must be aligned"),
     (_linear(bias=P + 1, flags=BIAS_16), "bias must be aligned"),
@@ -69,20 +74,40 @@ def _gated_backward(**over):
     (_linear_backward(dz=None), r"nil pointer \(dz\)"),
     (_linear_backward(act=0), "dz must be nil"),
     (_linear_backward(act=0, flags=D_F32, dz=None), r"nil pointer \(dz\)"),
-    (_linear_backward(dz=P, dy=P, z=P + 4096, lddz=32), "dz in dY's memory"),
-    (_linear_backward(dz=P, dy=P, flags=D_F32, z=P + 4096), "dz in dY's memory"),
-    (_linear_backward(dz=P, z=P, dy=P + 4096, lddz=32), "dz in z's memory"),
+    (_linear_backward(dz=_at(0), lddz=32), "dz in dY's memory"),
+    (_linear_backward(dz=_at(0), flags=D_F32), "dz in dY's memory"),
+    (_linear_backward(dz=_at(3), lddz=32), "dz in z's memory"),
     (_linear_backward(b=None), r"nil pointer \(b\)"),
     (_linear_backward(a=None), r"nil pointer \(a\)"),
     (_linear_backward(ldda=8), "pitch 8 of da is below"),
     (_linear_backward(dbias=P + 2), "dbias must be 4-byte aligned"),
-    (_gated_backward(dg=P + 8192), "dg and du share memory"),
+    (_gated_backward(dg=_at(7)), "dg and du share memory"),
     (_gated_backward(dg=None), r"nil pointer \(dg\)"),
     (_gated_backward(dwg=None), "dwg and dwu are given together"),
-    (_gated_backward(dg=P, lddg=32), "in an input's memory needs its pitch"),
+    (_gated_backward(dg=_at(0), lddg=32), "in an input's memory needs its pitch"),
     (_gated_backward(lddx=8), "pitch 8 of dx is below"),
     (_gated_backward(wg=None), r"nil pointer \(wg\)"),
     (_gated_backward(flags=BIAS_16), "unknown flags 0x20"),
+    # An output over an input or another output, but for the allowed places.
+    (_linear(d=_at(0)), "d lies over another"),
+    (_linear(z=_at(2), ldz=24), "d lies over another"),
+    (_linear(residual=P, ldres=24, z=P, ldz=24), "z lies over another"),
+    (_gated(g=_at(3), u=_at(4), ldg=24, ldu=24), "h lies over another"),
+    (_gated(g=_at(4), u=_at(4), ldg=24, ldu=24), "g lies over another"),
+    (_gated(g=_at(5), u=_at(1), ldg=24, ldu=24), "u lies over another"),
+    (_linear_backward(da=_at(1)), "da lies over another"),
+    (_linear_backward(da=_at(4)), "dz lies over another"),
+    (_linear_backward(db=_at(2)), "db lies over another"),
+    (_linear_backward(dbias=_at(2)), "dbias lies over another"),
+    (_gated_backward(dx=_at(1)), "dx lies over another"),
+    (_gated_backward(dwu=_at(9)), "dwg lies over another"),
+    (_gated_backward(dwg=_at(2)), "dwg lies over another"),
+    (_gated_backward(du=_at(8)), "du lies over another"),
+    # Contractions that a bounded wait would not outlast.
+    (_linear(K=2 ** 26 + 8, lda=2 ** 26 + 8), "contraction over 67108872 is too long"),
+    (_gated(K=2 ** 27, ldx=2 ** 27), "contraction over 134217728 is too long"),
+    (_linear_backward(M=2 ** 26 + 1), "contraction over 67108865 is too long"),
+    (_gated_backward(M=2 ** 26 + 1), "contraction over 67108865 is too long"),
 ], ids=lambda v: v[0] if isinstance(v, tuple) else None)
 def test_refusals(cudair, call, message):
     name, args = call
