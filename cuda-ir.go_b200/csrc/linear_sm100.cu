@@ -137,6 +137,7 @@ struct Index {
 __device__ __forceinline__ int job_of(const PairArgs &p, int t) {
     return (t >= p.first[1] ? 1 : 0) + (t >= p.first[2] ? 1 : 0);
 }
+
 __device__ __forceinline__ void drain_wait(uint64_t *bar, uint32_t parity, unsigned int *status) {
     int never = 0;
     mbar_wait(bar, parity, &never, status, kSiteDrain);
@@ -185,8 +186,9 @@ constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
 // accumulator was waited for.  The residual's further columns are requested while the
 // ones before them are worked on.
 template <bool GATED, bool bf16>
-__device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row, int n0, bool live,
-                                               bool any, Row32 &next, const float (&bias)[kWarpCols<GATED> / 32], uint32_t acc_empty) {
+__device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row,
+                                               int n0, bool live, bool any, Row32 &next,
+                                               const float (&bias)[kWarpCols<GATED> / 32], uint32_t acc_empty) {
 #pragma unroll 1
     for (int c = 0; c < kWarpCols<GATED>; c += 32) {
         const int col = n0 + c;
@@ -222,8 +224,8 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
 #pragma unroll
                 for (int j = 0; j < 32; j += 2)
                     unpair(add2(pair(v[j], v[j + 1]),
-                               pair(__shfl_sync(0xFFFFFFFFu, mine, j), __shfl_sync(0xFFFFFFFFu, mine, j + 1))),
-                          v[j], v[j + 1]);
+                                pair(__shfl_sync(0xFFFFFFFFu, mine, j), __shfl_sync(0xFFFFFFFFu, mine, j + 1))),
+                           v[j], v[j + 1]);
             }
             if (p.z[0].p && live) store_row32(p.z[0], row, col, job.N, bf16, v);
             if (p.act != CUDAIR_ACT_NONE)
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     using Cfg = PairCfg<NB>;
     constexpr int STAGES = Cfg::STAGES;
     constexpr int BLOCK_N = GATED ? BN / 2 : BN;  // columns of D per accumulator block
-    constexpr int TILE_N = NB * BLOCK_N;        // ... and per tile
+    constexpr int TILE_N = NB * BLOCK_N;          // ... and per tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t *smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);  // same offset in both CTAs
@@ -371,10 +373,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 else
                     ok = load_tile(Index<2>{}, t - p.first[2]);
             }
-            if (!ok) give_up();
-            // This CTA's copies complete on the even CTA's barriers, which
-            // only that CTA can wait on: give them time to land.
-            if (!ok) spin_ns(2000000);
+            if (!ok) {
+                give_up();
+                // This CTA's copies complete on the even CTA's barriers, which
+                // only that CTA can wait on: give them time to land.
+                spin_ns(2000000);
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -519,12 +523,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!GATED && p.residual.p && live && col0 < job.N)
                     fetch_row32(p.residual, row, col0, job.N, res);
                 if (num_kb > 0) {
-                    if (!mbar_wait(&acc_full[bar], acc_phase, abort_flag, p.status, kSiteEpilogueAccFull)) {
+                    // The warp stops as one: TMEM loads are warp-wide.
+                    if (!__all_sync(0xFFFFFFFFu, mbar_wait(&acc_full[bar], acc_phase, abort_flag, p.status,
+                                                           kSiteEpilogueAccFull))) {
                         give_up();
                         aborted = true;
                         break;
                     }
-                    __syncwarp();
                     tc_fence_after_sync();
                 }
                 const uint32_t mine_empty = mapa_shared(smem_u32(&acc_empty[bar]), 0);

@@ -258,6 +258,12 @@ def test_nan_and_inf_stay_in_their_row_and_column(dev, cudair, M):
         zz = torch.tensor([[-6e4, -3e4, -300.0, -100.0, 100.0, 300.0, 3e4, 6e4]], device=dev).half()
         kernels.linear_backward(dy, one[:1], one, z=zz, dz=dz, da=torch.empty_like(dz), act=act)
         assert dz[0].tolist() == [0, 0, 0, 0, 1, 1, 1, 1], (act, dz)
+    # An infinite pre-activation stays infinite.
+    k0, inf = torch.zeros(M, 0, device=dev).half(), torch.full((8,), float("inf"), device=dev)
+    for act in ("relu", "silu", "gelu", "gelu_tanh"):
+        y = torch.empty(M, 8, device=dev)
+        kernels.linear(k0, torch.zeros(0, 8, device=dev).half(), y, bias=inf, act=act)
+        assert bool((y == float("inf")).all()), act
     zz = torch.full((1, 8), 3e38, device=dev).bfloat16()
     dz = torch.empty_like(zz)
     for sign in (1, -1):
@@ -441,3 +447,84 @@ def test_64_bit_offsets(dev, cudair):
     kernels.linear_backward(y, x, w, z=y, dz=dz, db=db, act="silu", b_trans=True)
     kernels.linear_backward(small, x.contiguous(), w, z=small, dz=dz2, db=db2, act="silu", b_trans=True)
     assert torch.equal(dz, dz2) and torch.equal(db, db2)
+
+
+def test_many_sizes_at_once(dev, cudair):
+    """Calls of every tile height, plain and gated, kept in flight together on
+    four streams: each as when it runs alone."""
+    import torch
+    from cudair import kernels
+    bf = torch.bfloat16
+    gen = _gen(dev, 77)
+    calls = []
+    for M in (1, 20, 40, 64, 90, 128, 200, 500):
+        for K, N, gated in ((2048, 640, False), (512, 1408, True), (1088, 4096, False)):
+            x, w, w2 = normal(gen, M, K, bf, dev), _weight(gen, N, K, bf, dev, True), _weight(gen, N, K, bf, dev, True)
+            y = torch.empty(M, N, dtype=bf, device=dev)
+
+            def call(stream, x=x, w=w, w2=w2, y=y, gated=gated):
+                if gated:
+                    kernels.gated(x, w, w2, y, b_trans=True, stream=stream)
+                else:
+                    kernels.linear(x, w, y, act="gelu", b_trans=True, stream=stream)
+            calls.append((call, y))
+    want = []
+    for call, y in calls:
+        call(None)
+        torch.cuda.synchronize()
+        want.append(y.clone())
+        y.fill_(9.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for turn in range(6):
+        for i, (call, _) in enumerate(calls):
+            call(streams[(i + turn) % 4] if turn % 2 else streams[i % 4])
+        torch.cuda.synchronize()
+        for (_, y), w in zip(calls, want):
+            assert torch.equal(y, w)
+            y.fill_(9.0)
+        torch.cuda.synchronize()
+    assert kernels.wait_status(clear=True) == 0
+
+
+_CAPTURE = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from cudair import kernels
+bf, dev = torch.bfloat16, "cuda"
+r = lambda *s: torch.randn(*s, device=dev).to(bf)
+M, N, K = (40, 256, 128) if sys.argv[2] == "few" else (1304, 1104, 1200)
+x, w, w2, y, z, g, u, h = r(M, K), r(N, K), r(N, K), r(M, N), r(M, N), r(M, N), r(M, N), r(M, N)
+outs = [torch.empty_like(t) for t in (x, w, w2, x, w, y, y, y)]
+db = torch.empty(N, device=dev)
+def run():
+    kernels.gated(x, w, w2, outs[5], act="silu", b_trans=True)
+    kernels.linear(x, w, outs[6], act="gelu", b_trans=True)
+    kernels.linear_backward(y, x, w, z=z, dz=outs[7], da=outs[0], db=outs[1], dbias=db, act="gelu", b_trans=True)
+    kernels.gated_backward(h, x, w, w2, g, u, g, u, dx=outs[3], dwg=outs[2], dwu=outs[4], b_trans=True)
+torch.cuda.synchronize()
+g0, u0 = g.clone(), u.clone()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    run()  # the library's first call in this process
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in outs + [db]]
+g.copy_(g0); u.copy_(u0)
+run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, outs + [db]))
+assert kernels.wait_status() == 0
+print("captured")
+"""
+
+
+@pytest.mark.parametrize("size", ["few", "many"])
+def test_first_call_may_be_captured(dev, cudair, size):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _CAPTURE, os.path.join(here, "cuda-ir.go_b200"), size],
+                       capture_output=True, text=True, timeout=240)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
