@@ -58,11 +58,10 @@ constexpr uint32_t A_STAGE = 128 * BK * 2;
 constexpr uint32_t BAR_BYTES = 256 + 512;  // barriers, and the jobs' arguments
 constexpr int GROUP_M = 8;  // row-blocks visited together (A and B panels shared in L2)
 
-// A tile takes NB accumulator blocks of BN columns (the MMA's N).  NB = 1: two
-// accumulators that alternate.  NB = 2: one of 512 columns that fills TMEM, for a
-// quarter fewer operand bytes per flop.  (BN = 128 tiles for outputs of few
-// tiles gain nothing: a 256 x 128 MMA takes as long as a 256 x 256 one, 512 x
-// 4096 x 4096 26.1 against 26.4 us.)
+// A tile takes NB accumulator blocks of bn columns (the MMA's N, at most BN).
+// NB = 1: two accumulators that alternate.  NB = 2: one of up to 512 columns
+// that fills TMEM, for a quarter fewer operand bytes per flop.  bn is chosen per
+// call so that the tiles fill whole waves (see tile_time).
 constexpr int BN = 256;
 template <int NB>
 struct PairCfg {
@@ -97,6 +96,7 @@ struct JobArgs {
     uint32_t idesc;
     int per_group;       // tiles of a group of GROUP_M row-blocks
     Div group, last;     // by per_group; by the row-blocks of the last group
+    uint32_t bytes;      // both CTAs' copies of a k-block
 };
 static_assert(sizeof(JobArgs) % 4 == 0, "copied by words");
 
@@ -110,6 +110,7 @@ struct PairArgs {
     int first[kMaxJobs + 1];  // a job's first tile; the end
     int own, more;            // tiles of job 0 of every pair; pairs that take one more
     int rounds;
+    int bn;  // columns of an accumulator block, a multiple of 32 (gated: of 64)
     int act;
     Mat z[2], residual;
     const void *bias;
@@ -175,30 +176,30 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// Columns of D that one epilogue warp takes of an accumulator block: two warps
-// share the block's 32 rows of a TMEM lane quarter.
+// Two warps share an accumulator block's 32 rows of a TMEM lane quarter; each
+// takes about half of its columns of D, in chunks of 32 and at most this many.
 template <bool GATED>
 constexpr int kWarpCols = (GATED ? BN / 2 : BN) / (EPI_WARPS / 4);
 
-// One warp's 32 rows (one per lane) and kWarpCols columns from n0 on; t_row is
+// One warp's 32 rows (one per lane) and `cols` columns from n0 on; t_row is
 // where they start in TMEM.  `next` holds the residual's first 32 columns, and lane
 // l of `bias` the warp's columns l, l + 32, ...: both were requested before the
 // accumulator was waited for.  The residual's further columns are requested while the
 // ones before them are worked on.
 template <bool GATED, bool bf16>
 __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs &job, uint32_t t_row, int row,
-                                               int n0, bool live, bool any, Row32 &next,
+                                               int n0, int cols, bool live, bool any, Row32 &next,
                                                const float (&bias)[kWarpCols<GATED> / 32], uint32_t acc_empty) {
 #pragma unroll 1
-    for (int c = 0; c < kWarpCols<GATED>; c += 32) {
+    for (int c = 0; c < cols; c += 32) {
         const int col = n0 + c;
         if (col >= job.N) break;
         float v[32], u[GATED ? 32 : 1];
         load_acc(any, t_row + c, v);
-        if constexpr (GATED) load_acc(any, t_row + BN / 2 + c, u);
+        if constexpr (GATED) load_acc(any, t_row + p.bn / 2 + c, u);
         // The last columns are read: the block goes back to the MMA warp while
         // they are worked on.
-        if (any && (c + 32 >= kWarpCols<GATED> || col + 32 >= job.N)) {
+        if (any && (c + 32 >= cols || col + 32 >= job.N)) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane_id() == 0) mbar_arrive_cluster_relaxed(acc_empty);
@@ -235,7 +236,7 @@ __device__ __forceinline__ void epilogue_block(const PairArgs &p, const JobArgs 
                 });
             if (p.residual.p && live) {
                 add_row32(next, p.residual.f32, bf16, v);
-                if (c + 32 < kWarpCols<GATED> && col + 32 < job.N)
+                if (c + 32 < cols && col + 32 < job.N)
                     fetch_row32(p.residual, row, col + 32, job.N, next);
             }
         }
@@ -248,8 +249,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     product_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ PairArgs p) {
     using Cfg = PairCfg<NB>;
     constexpr int STAGES = Cfg::STAGES;
-    constexpr int BLOCK_N = GATED ? BN / 2 : BN;  // columns of D per accumulator block
-    constexpr int TILE_N = NB * BLOCK_N;          // ... and per tile
+    const int half = p.bn / 2;                  // a CTA's columns of B per block
+    const int block_n = GATED ? half : p.bn;    // columns of D per accumulator block
+    const int tile_n = NB * block_n;            // ... and per tile
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = smem_u32(smem_raw);
     uint8_t *smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);  // same offset in both CTAs
@@ -328,12 +330,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // A block takes the first half of its columns of B from the even
                 // CTA, the others from the odd one: of one weight, or (gated)
                 // of the two.
-                const int n_mine = n_blk * TILE_N + (GATED ? 0 : BN / 2 * static_cast<int>(rank));
+                const int n_mine = n_blk * tile_n + (GATED ? 0 : half * static_cast<int>(rank));
                 int k0 = 0;
                 for (int kb = 0; kb < num_kb; ++kb, k0 += BK) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteProducerEmpty)) return false;
                     const uint32_t full_even = mapa_shared(smem_u32(&full[stage]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::STAGE);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], job.bytes);
                     if (!GATED && kb == job.num_kb) {  // the second contraction
                         ++ma;
                         ++mb;
@@ -349,11 +351,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int h = 0; h < NB; ++h) {
                         uint8_t *dh = db + h * Cfg::B_BLOCK;
-                        const int n = n_mine + h * BLOCK_N;
+                        const int n = n_mine + h * block_n;
                         if (job.b_mn) {
-#pragma unroll
-                            for (int x = 0; x < BN / 2; x += 64)
-                                tma_load_2d_pair(dh + x * BK * 2, mb, full_even, n + x, k0, policy);
+                            tma_load_2d_pair(dh, mb, full_even, n, k0, policy);
+                            if (half > 64) tma_load_2d_pair(dh + 64 * BK * 2, mb, full_even, n + 64, k0, policy);
                         } else {
                             tma_load_2d_pair(dh, mb, full_even, k0, n, policy);
                         }
@@ -492,7 +493,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         // ---------------- epilogue (warps 2..9, both CTAs) ----------------
         grid_dependency_wait();  // the outputs may be the preceding kernel's inputs
         const uint32_t q = warp & 3u;  // the TMEM lane quarter this warp may read
-        const int side = static_cast<int>(warp - 2u) / 4;  // which of the quarter's warps
+        // Which of the quarter's warps this is, and its columns of a block.
+        const int side = static_cast<int>(warp - 2u) / 4;
+        const int split_at = (block_n / 32 + 1) / 2 * 32;
+        const int first_col = side ? split_at : 0, cols = side ? block_n - split_at : split_at;
         uint32_t acc = 0, acc_phase = 0;
         for (int i = 0, t; (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
             const int j = job_of(p, t);
@@ -502,13 +506,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             tile_coords(job, t - p.first[j], m_blk, n_blk);
             const int row0 = m_blk * PM + 128 * static_cast<int>(rank) + static_cast<int>(q * 32);
             const int row = row0 + static_cast<int>(lane);
-            const int n0 = n_blk * TILE_N;
+            const int n0 = n_blk * tile_n;
             const bool live = row < job.M;
             bool aborted = false;
 #pragma unroll 1
             for (int h = 0; h < NB; ++h) {
                 const uint32_t bar = acc + h;  // NB = 2: block h's own barriers
-                const int col0 = n0 + h * BLOCK_N + side * kWarpCols<GATED>;
+                const int col0 = n0 + h * block_n + first_col;
                 Row32 res;
                 float bias[kWarpCols<GATED> / 32] = {};
                 if (!GATED && p.bias) {
@@ -533,9 +537,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc_fence_after_sync();
                 }
                 const uint32_t mine_empty = mapa_shared(smem_u32(&acc_empty[bar]), 0);
-                const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + side * kWarpCols<GATED>;
+                const uint32_t t_row = tmem_base + ((q * 32u) << 16) + bar * BN + first_col;
                 if (row0 < job.M && col0 < job.N)  // the whole warp: TMEM loads are warp-wide
-                    epilogue_block<GATED, BF16>(p, job, t_row, row, col0, live, num_kb > 0, res, bias, mine_empty);
+                    epilogue_block<GATED, BF16>(p, job, t_row, row, col0, cols, live, num_kb > 0, res, bias,
+                                                mine_empty);
                 else if (num_kb > 0 && lane == 0)  // nothing of it lies in D
                     mbar_arrive_cluster_relaxed(mine_empty);
                 __syncwarp();
@@ -619,7 +624,9 @@ int resident_pairs(int sm_count, int *pairs) {
             (e = prepare_kernel<false, 2, false>(sm_count, &n)) != cudaSuccess ||
             (e = prepare_kernel<false, 2, true>(sm_count, &n)) != cudaSuccess ||
             (e = prepare_kernel<true, 1, false>(sm_count, &n)) != cudaSuccess ||
-            (e = prepare_kernel<true, 1, true>(sm_count, &n)) != cudaSuccess)
+            (e = prepare_kernel<true, 1, true>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<true, 2, false>(sm_count, &n)) != cudaSuccess ||
+            (e = prepare_kernel<true, 2, true>(sm_count, &n)) != cudaSuccess)
             return cuda_error(e, "product_pair_kernel set-up");
         if (n < 1) return set_error(CUDAIR_ERR_CUDA, "cudair: no CTA pair of the linear kernels fits this device");
         g_pairs[dev] = n;
@@ -628,14 +635,30 @@ int resident_pairs(int sm_count, int *pairs) {
     return CUDAIR_OK;
 }
 
-// A tile's time in microseconds, fitted on B200: 8192^3, 14 waves of 256 x 256
-// tiles 898 us against 7 of 256 x 512 855 us, back to back; 2048 x 14336 x 4096, 7
-// waves 165 us against 4 waves 198 us.  With A's rows along memory (weight
-// gradients) the narrow tile costs more: dWg, dWu of 14336 x 4096 over 4096
-// rows, 25 waves 777 us against 13 waves 736 us.
-double tile_time(const Job &j, int nb) {
-    const double k = static_cast<double>(j.K) * j.parts;
-    return nb == 2 ? 0.0112 * k + 4.5 : (j.a[0].mn ? 0.0066 : 0.0059) * k + 0.2;
+// The width of a tile, NB blocks of bn accumulator columns, and the time of one
+// of its k-blocks in microseconds, in four waves and in a single one, which runs at
+// a higher clock (72 tiles of 2048 rows a wave, K 1024 and 4096).  Below 192 columns
+// a tile gains nothing more: 0.30 for 160 columns and 0.29 for 128.  What the widths are for is whole
+// waves: 800 x 5504 x 6208 is 88 tiles of 256 columns, two waves on 74 pairs, but
+// 60 of 384.
+struct Width {
+    int nb, bn;
+    double many, single;
+};
+constexpr Width kWidths[] = {{1, 256, 0.371, 0.319}, {1, 224, 0.343, 0.317}, {1, 192, 0.323, 0.308},
+                             {2, 256, 0.731, 0.673}, {2, 224, 0.639, 0.560}, {2, 192, 0.551, 0.473}};
+
+// A tile's time.  Rows of B along memory come in twice as many copies, rows of
+// A and B (weight gradients) more still, which narrow tiles feel.  A tile of
+// two blocks ends with an epilogue that nothing hides.
+double tile_time(const Job &j, const Width &w, bool gated, bool one_wave) {
+    double block = one_wave ? w.single : w.many;
+    if (w.nb == 1 && j.a[0].mn)
+        block = one_wave ? 0.404 : 0.42;
+    else if (w.nb == 1 && j.b[0].mn)
+        block *= 1.07;
+    const double kb = static_cast<double>((j.K + BK - 1) / BK * j.parts);
+    return kb * block + (w.nb == 1 ? 0.2 : gated ? 6.0 : 3.5);
 }
 
 // How the tiles of all jobs are dealt out (see PairArgs), and how long that
@@ -646,13 +669,14 @@ struct Deal {
     int64_t rounds = 0;
     double time = 0.0;
 };
-Deal deal(const Product &p, int nb, int pairs) {
+Deal deal(const Product &p, const Width &w, int pairs) {
     Deal d;
+    // Longest contractions first.
     for (int i = 0; i < p.jobs; ++i) d.order[i] = i;
+    auto depth = [&](int i) { return p.job[d.order[i]].K * p.job[d.order[i]].parts; };
     for (int i = 1; i < p.jobs; ++i)
-        for (int k = i; k > 0 && tile_time(p.job[d.order[k]], nb) > tile_time(p.job[d.order[k - 1]], nb); --k)
-            std::swap(d.order[k], d.order[k - 1]);
-    const int64_t tile_n = static_cast<int64_t>(BN) * nb / p.tiles_of_b();
+        for (int k = i; k > 0 && depth(k) > depth(k - 1); --k) std::swap(d.order[k], d.order[k - 1]);
+    const int64_t tile_n = static_cast<int64_t>(w.bn) * w.nb / p.tiles_of_b();
     d.first[0] = 0;
     for (int i = 0; i < kMaxJobs; ++i) {
         int64_t n = 0;
@@ -664,7 +688,9 @@ Deal deal(const Product &p, int nb, int pairs) {
     }
     const int64_t C = d.first[kMaxJobs] < pairs ? d.first[kMaxJobs] : pairs;
     const int64_t n0 = d.first[1], n1 = d.first[kMaxJobs] - n0, more = n0 % C;
-    const double a = tile_time(p.job[d.order[0]], nb), b = p.jobs > 1 ? tile_time(p.job[d.order[1]], nb) : 0.0;
+    const bool one_wave = d.first[kMaxJobs] <= pairs;
+    const double a = tile_time(p.job[d.order[0]], w, p.gated, one_wave);
+    const double b = p.jobs > 1 ? tile_time(p.job[d.order[1]], w, p.gated, one_wave) : 0.0;
     const double own = static_cast<double>(n0 / C) * a;
     if (n1 == 0 || more == 0) {
         d.time = own + (more ? a : 0.0) + static_cast<double>((n1 + C - 1) / C) * b;
@@ -685,6 +711,20 @@ Deal deal(const Product &p, int nb, int pairs) {
     }
     if (d.time == 1e30) d.time = own + a;  // the short tiles end before one more long one
     return d;
+}
+
+Deal best_deal(const Product &p, int pairs, Width *width) {
+    Deal best;
+    best.time = 1e300;
+    for (const Width &w : kWidths) {
+        if (p.gated && w.bn % 64) continue;  // its columns of D are half as many
+        const Deal d = deal(p, w, pairs);
+        if (d.time < best.time) {
+            best = d;
+            *width = w;
+        }
+    }
+    return best;
 }
 
 template <bool GATED, int NB>
@@ -715,8 +755,8 @@ int product_pair_time(const Product &p, int sm_count, double *us) {
     int pairs = 0;
     const int rc = resident_pairs(sm_count, &pairs);
     if (rc != CUDAIR_OK) return rc;
-    const double narrow = deal(p, 1, pairs).time, wide = p.gated ? narrow : deal(p, 2, pairs).time;
-    *us = (p.gated ? 7.5 : 6.0) + (narrow < wide ? narrow : wide);  // launch, set-up and the last epilogue
+    Width w;
+    *us = (p.gated ? 7.5 : 6.0) + best_deal(p, pairs, &w).time;  // launch, set-up and the last epilogue
     return CUDAIR_OK;
 }
 
@@ -724,23 +764,14 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     int pairs = 0;
     int rc = resident_pairs(sm_count, &pairs);
     if (rc != CUDAIR_OK) return rc;
-    // gated keeps 256 x 256 tiles: its epilogue is long enough to want two
-    // accumulators (4096 x 14336 x 4096 719 against 726 us, 744 against 781 us with
-    // G and U stored).
-    Deal d = deal(p, 1, pairs);
-    int nb = 1;
-    if (!p.gated) {
-        const Deal wide = deal(p, 2, pairs);
-        if (wide.time < d.time) {
-            d = wide;
-            nb = 2;
-        }
-    }
+    Width w;
+    const Deal d = best_deal(p, pairs, &w);
     if (d.first[kMaxJobs] > INT32_MAX / 2)
         return set_error(CUDAIR_ERR_INVALID, "cudair: linear: %lld tiles are too many", (long long)d.first[kMaxJobs]);
     alignas(64) Maps maps = {};
     PairArgs args = {};
-    const int tile_n = BN * nb / p.tiles_of_b();
+    const int tile_n = w.bn * w.nb / p.tiles_of_b();
+    args.bn = w.bn;
     for (int i = 0; i <= kMaxJobs; ++i) args.first[i] = static_cast<int>(d.first[i]);
     args.rounds = static_cast<int>(d.rounds);
     const int C = args.first[kMaxJobs] < pairs ? args.first[kMaxJobs] : pairs;
@@ -760,13 +791,16 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
         o.last = divide_by((o.num_m - 1) % GROUP_M + 1);
         o.a_mn = j.a[0].mn;
         o.b_mn = j.b[0].mn;
-        o.idesc = idesc_f16_f32(PM, BN, j.a[0].mn, j.b[0].mn, p.bf16);
+        o.idesc = idesc_f16_f32(PM, static_cast<uint32_t>(w.bn), j.a[0].mn, j.b[0].mn, p.bf16);
+        // Rows of B along memory come in whole 64-column boxes.
+        const int cols = j.b[0].mn ? (w.bn / 2 + 63) / 64 * 64 : w.bn / 2;
+        o.bytes = 2 * (A_STAGE + static_cast<uint32_t>(w.nb * cols) * BK * 2);
         o.d = mat_of(j.d);
         if (j.K == 0) continue;
         for (int k = 0; k < j.parts; ++k)
             if ((rc = operand_map(&maps.a[i][k], j.a[k], j.M, j.K, 128, p.bf16)) != CUDAIR_OK) return rc;
         for (int k = 0; k < (p.gated ? 2 : j.parts); ++k)
-            if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, BN / 2, p.bf16)) != CUDAIR_OK) return rc;
+            if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, static_cast<uint32_t>(w.bn / 2), p.bf16)) != CUDAIR_OK) return rc;
     }
     args.act = p.act;
     for (int i = 0; i < 2; ++i) args.z[i] = mat_of(p.z[i]);
@@ -775,9 +809,11 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
     args.bias16 = p.bias16;
     args.status = status;
     const bool pdl = p.pdl();
-    const cudaError_t e = p.gated ? launch_pair<true, 1>(maps, args, pairs, p.bf16, pdl, stream)
-                          : nb == 2 ? launch_pair<false, 2>(maps, args, pairs, p.bf16, pdl, stream)
-                                    : launch_pair<false, 1>(maps, args, pairs, p.bf16, pdl, stream);
+    const bool wide = w.nb == 2;
+    const cudaError_t e = p.gated ? (wide ? launch_pair<true, 2>(maps, args, pairs, p.bf16, pdl, stream)
+                                          : launch_pair<true, 1>(maps, args, pairs, p.bf16, pdl, stream))
+                                  : (wide ? launch_pair<false, 2>(maps, args, pairs, p.bf16, pdl, stream)
+                                          : launch_pair<false, 1>(maps, args, pairs, p.bf16, pdl, stream));
     return e == cudaSuccess ? CUDAIR_OK : cuda_error(e, "product_pair_kernel launch");
 }
 
