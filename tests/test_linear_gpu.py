@@ -528,3 +528,39 @@ def test_first_call_may_be_captured(dev, cudair, size):
     r = subprocess.run([sys.executable, "-c", _CAPTURE, os.path.join(here, "cuda-ir.go_b200"), size],
                        capture_output=True, text=True, timeout=240)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_wrapper_refusals(dev, cudair):
+    import torch
+    from cudair import kernels
+    from cudair._lib import CudairError
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device=dev)  # noqa: E731
+    a, b, d = h(4, 16), h(16, 24), h(4, 24)
+    for message, call in [
+            ("a must be a float16 or bfloat16 tensor", lambda: kernels.linear(a.float(), b, d)),
+            ("a must be a float16 or bfloat16 tensor", lambda: kernels.linear(None, b, d)),
+            ("a and b must be matrices", lambda: kernels.linear(a, None, d)),
+            ("b must be torch.float16, got torch.bfloat16", lambda: kernels.linear(a, b.bfloat16(), d)),
+            ("b must be 16 x 20", lambda: kernels.linear(a, h(18, 20), d)),
+            ("d must be 4 x 24", lambda: kernels.linear(a, b, h(4, 25))),
+            ("d must be torch.float16 or torch.float32", lambda: kernels.linear(a, b, d.bfloat16())),
+            ("d needs unit inner stride", lambda: kernels.linear(a, b, h(24, 4).t())),
+            ("d must be a CUDA tensor", lambda: kernels.linear(a, b, d.cpu())),
+            ("pitch 25 of d must be a multiple of 8", lambda: kernels.linear(a, b, h(4, 25)[:, :24])),
+            ("bias must have 24 consecutive values", lambda: kernels.linear(a, b, d, bias=h(23))),
+            ("bias must have 24 consecutive values", lambda: kernels.linear(a, b, d, bias=h(48)[::2])),
+            ("residual must be torch.float16", lambda: kernels.linear(a, b, d, residual=d.float())),
+            ("act must be one of none, relu, gelu, gelu_tanh, silu", lambda: kernels.linear(a, b, d, act="tanh")),
+            ("d lies over another matrix", lambda: kernels.linear(h(4, 24), h(24, 24), d, z=d)),
+            ("g and u are given together", lambda: kernels.gated(a, b, b, d, g=h(4, 24))),
+            ("wu must be 16 x 24", lambda: kernels.gated(a, b, h(16, 25), d)),
+            (r"nil pointer \(dz\)", lambda: kernels.linear_backward(d, a, b, z=h(4, 24), da=h(4, 16), act="relu")),
+            ("dz must be nil", lambda: kernels.linear_backward(d, a, b, dz=h(4, 24), da=h(4, 16))),
+            ("dbias must be torch.float32", lambda: kernels.linear_backward(d, a, b, dbias=h(24))),
+            ("dwg and dwu are given together", lambda: kernels.gated_backward(
+                d, a, b, b, h(4, 24), h(4, 24), h(4, 24), h(4, 24), dwg=h(16, 24)))]:
+        with pytest.raises(CudairError, match=message):
+            call()
+    # One row needs no pitch of its own.
+    kernels.linear(h(1, 15), h(15, 24), h(1, 24))
+    torch.cuda.synchronize()
