@@ -25,10 +25,18 @@
 //
 // What bounds it: the tensor pipe, for the sizes it is meant for (M > 128;
 // 2 M N K flop against 2 (MK + NK + MN) bytes).  Roles, ring and bounded waits
-// are those of gemm_sm100.cu: warp 0 TMA producer, warp 1 TMEM owner and MMA
-// issuer (even CTA), warps 2-9 epilogue (two per lane quarter).  Two
-// accumulators of 256 columns alternate, so a tile's epilogue runs under the
-// next tile's mainloop; or one of 512 columns is handed over in halves.
+// are those of gemm_sm100.cu, with a second producer: warp 0 loads A, warp 10 loads B
+// (one thread issuing the four copies of a k-block whose operands both have rows along
+// memory fell behind: weight gradients of 5632 x 2048 over 1024 rows 42.6 -> 37
+// us), warp 1 TMEM owner and MMA issuer (even CTA), warps 2-9 epilogue (two
+// per lane quarter).  Two accumulators of 256 columns alternate, so a tile's
+// epilogue runs under the next tile's mainloop; or one of 512 columns is handed
+// over in halves.
+//
+// Below that bound, what limits a k-block is the way from L2: 32 KB into an SM
+// in 0.29 us with few SMs busy (59 bytes a clock), 0.37 us with all (13 TB/s
+// in all).  So outputs of few tiles stay short of a kernel that shares copies
+// between CTAs (512 x 4096 x 4096: 26 us).
 //
 // The epilogue writes each thread's row straight from registers, 32 bytes a
 // store (a whole sector): no staging in shared memory, which goes to the ring
@@ -52,7 +60,7 @@ namespace ffn {
 
 constexpr int BK = 64;
 constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int THREADS = 64 + 32 * EPI_WARPS + 32;  // the last warp loads B
 constexpr int PM = 256;  // rows per pair tile, 128 per CTA
 constexpr uint32_t A_STAGE = 128 * BK * 2;
 constexpr uint32_t BAR_BYTES = 256 + 512;  // barriers, and the jobs' arguments
@@ -306,24 +314,26 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     auto give_up = [&]() { st_shared_cluster_u32(peer_abort, 1u); };
 
-    if (warp == 0) {
-        // ---------------- TMA producer (both CTAs) ----------------
+    if (warp == 0 || warp == 2 + EPI_WARPS) {
+        // ---------------- TMA producers (both CTAs): A, B ----------------
         if (lane == 0) {
             grid_dependency_wait();
             const uint64_t policy = l2_policy_evict_normal();
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            // One tile of job J.  J is a template parameter: with an indexed
-            // tensor map the compiler cannot tell that its address is uniform,
-            // as the copy instruction needs, and the loop that makes it so sets the
-            // pace (1024 x 4096 x 8192: 60 us against 52).
-            auto load_tile = [&](auto tag, int t) -> bool {
+            // One operand of one tile of job J.  Both are template parameters:
+            // with an indexed tensor map, or copies under a condition of the
+            // thread's, the compiler cannot tell that what the copy instruction needs
+            // is uniform, and the loop that makes it so sets the pace (1024 x
+            // 4096 x 8192: 60 us against 52).
+            auto load_tile = [&](auto operand, auto tag, int t) -> bool {
+                constexpr bool FOR_A = decltype(operand)::value == 0;
                 constexpr int J = decltype(tag)::value;
                 const JobArgs &job = p.job[J];
                 const int num_kb = job.all_kb;
                 int m_blk, n_blk;
                 tile_coords(job, t, m_blk, n_blk);
-                const CUtensorMap *ma = &maps.a[J][0], *mb = &maps.b[J][GATED ? rank : 0];
+                const CUtensorMap *map = FOR_A ? &maps.a[J][0] : &maps.b[J][GATED ? rank : 0];
                 // Rows and columns beyond the matrices arrive as zeros (the
                 // maps clip), so every stage carries the same bytes.
                 const int m_mine = m_blk * PM + 128 * static_cast<int>(rank);
@@ -335,28 +345,30 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int kb = 0; kb < num_kb; ++kb, k0 += BK) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, kSiteProducerEmpty)) return false;
                     const uint32_t full_even = mapa_shared(smem_u32(&full[stage]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], job.bytes);
+                    if (FOR_A && rank == 0) mbar_arrive_expect_tx(&full[stage], job.bytes);
                     if (!GATED && kb == job.num_kb) {  // the second contraction
-                        ++ma;
-                        ++mb;
+                        ++map;
                         k0 = 0;
                     }
-                    uint8_t *da = sA + stage * A_STAGE, *db = sB + stage * Cfg::B_STAGE;
-                    if (job.a_mn) {
-                        tma_load_2d_pair(da, ma, full_even, m_mine, k0, policy);
-                        tma_load_2d_pair(da + 64 * BK * 2, ma, full_even, m_mine + 64, k0, policy);
-                    } else {
-                        tma_load_2d_pair(da, ma, full_even, k0, m_mine, policy);
-                    }
-#pragma unroll
-                    for (int h = 0; h < NB; ++h) {
-                        uint8_t *dh = db + h * Cfg::B_BLOCK;
-                        const int n = n_mine + h * block_n;
-                        if (job.b_mn) {
-                            tma_load_2d_pair(dh, mb, full_even, n, k0, policy);
-                            if (half > 64) tma_load_2d_pair(dh + 64 * BK * 2, mb, full_even, n + 64, k0, policy);
+                    if constexpr (FOR_A) {
+                        uint8_t *da = sA + stage * A_STAGE;
+                        if (job.a_mn) {
+                            tma_load_2d_pair(da, map, full_even, m_mine, k0, policy);
+                            tma_load_2d_pair(da + 64 * BK * 2, map, full_even, m_mine + 64, k0, policy);
                         } else {
-                            tma_load_2d_pair(dh, mb, full_even, k0, n, policy);
+                            tma_load_2d_pair(da, map, full_even, k0, m_mine, policy);
+                        }
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < NB; ++h) {
+                            uint8_t *db = sB + stage * Cfg::B_STAGE + h * Cfg::B_BLOCK;
+                            const int n = n_mine + h * block_n;
+                            if (job.b_mn) {
+                                tma_load_2d_pair(db, map, full_even, n, k0, policy);
+                                if (half > 64) tma_load_2d_pair(db + 64 * BK * 2, map, full_even, n + 64, k0, policy);
+                            } else {
+                                tma_load_2d_pair(db, map, full_even, k0, n, policy);
+                            }
                         }
                     }
                     if (++stage == STAGES) {
@@ -366,14 +378,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 return true;
             };
-            for (int i = 0, t; ok && (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
-                if (GATED || t < p.first[1])
-                    ok = load_tile(Index<0>{}, t);
-                else if (t < p.first[2])
-                    ok = load_tile(Index<1>{}, t - p.first[1]);
-                else
-                    ok = load_tile(Index<2>{}, t - p.first[2]);
-            }
+            auto load_all = [&](auto operand) {
+                for (int i = 0, t; ok && (t = tile_of(p, i, cluster, num_clusters)) >= 0; ++i) {
+                    if (GATED || t < p.first[1])
+                        ok = load_tile(operand, Index<0>{}, t);
+                    else if (t < p.first[2])
+                        ok = load_tile(operand, Index<1>{}, t - p.first[1]);
+                    else
+                        ok = load_tile(operand, Index<2>{}, t - p.first[2]);
+                }
+            };
+            if (warp == 0)
+                load_all(Index<0>{});
+            else
+                load_all(Index<1>{});
             if (!ok) {
                 give_up();
                 // This CTA's copies complete on the even CTA's barriers, which
@@ -654,9 +672,9 @@ constexpr Width kWidths[] = {{1, 256, 0.371, 0.319}, {1, 224, 0.343, 0.317}, {1,
 double tile_time(const Job &j, const Width &w, bool gated, bool one_wave) {
     double block = one_wave ? w.single : w.many;
     if (w.nb == 1 && j.a[0].mn)
-        block = one_wave ? 0.404 : 0.42;
+        block = one_wave ? 0.36 : 0.40;
     else if (w.nb == 1 && j.b[0].mn)
-        block *= 1.07;
+        block *= 1.03;
     const double kb = static_cast<double>((j.K + BK - 1) / BK * j.parts);
     return kb * block + (w.nb == 1 ? 0.2 : gated ? 6.0 : 3.5);
 }
