@@ -818,7 +818,8 @@ int product_pair_launch(const Product &p, int sm_count, unsigned int *status, cu
         for (int k = 0; k < j.parts; ++k)
             if ((rc = operand_map(&maps.a[i][k], j.a[k], j.M, j.K, 128, p.bf16)) != CUDAIR_OK) return rc;
         for (int k = 0; k < (p.gated ? 2 : j.parts); ++k)
-            if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, static_cast<uint32_t>(w.bn / 2), p.bf16)) != CUDAIR_OK) return rc;
+            if ((rc = operand_map(&maps.b[i][k], j.b[k], j.N, j.K, static_cast<uint32_t>(w.bn / 2), p.bf16)) != CUDAIR_OK)
+                return rc;
     }
     args.act = p.act;
     for (int i = 0; i < 2; ++i) args.z[i] = mat_of(p.z[i]);
