@@ -561,6 +561,9 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         CUDAIR_TRY(check_distinct(op, "db", q->db, {q->a, q->b, q->dy, q->z, q->dbias}));
         CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->a, q->b, q->dy, q->z}));
     }
+    // Outputs that a call with an empty dimension still writes.
+    if (q->M > 0 && q->N > 0) CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->dz, q->dy, q->z}));
+    if (want_db) CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->db}));
 
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
@@ -660,6 +663,7 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->x, q->wg, q->wu, q->dh, q->g, q->u, q->dwu}));
         CUDAIR_TRY(check_distinct(op, "dwu", q->dwu, {q->x, q->wg, q->wu, q->dh, q->g, q->u}));
     }
+    if (want_dw) CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->dwu}));  // M = 0 writes them too
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
     const bool elementwise = q->M > 0 && q->N > 0;

@@ -99,8 +99,11 @@ def _gated_backward(**over):
     (_linear_backward(da=_at(4)), "dz lies over another"),
     (_linear_backward(db=_at(2)), "db lies over another"),
     (_linear_backward(dbias=_at(2)), "dbias lies over another"),
+    (_linear_backward(dbias=_at(4), K=0), "dbias lies over another"),
+    (_linear_backward(dbias=_at(6), M=0), "dbias lies over another"),
     (_gated_backward(dx=_at(1)), "dx lies over another"),
     (_gated_backward(dwu=_at(9)), "dwg lies over another"),
+    (_gated_backward(dwu=_at(9), M=0), "dwg lies over another"),
     (_gated_backward(dwg=_at(2)), "dwg lies over another"),
     (_gated_backward(du=_at(8)), "du lies over another"),
     # Contractions that a bounded wait would not outlast.
