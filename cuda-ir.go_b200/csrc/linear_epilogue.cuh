@@ -128,24 +128,38 @@ __device__ __forceinline__ float relu(float z) {
     return r;
 }
 
+// z held above -1e18 and below 1e18, a NaN kept.  There the activations and their
+// derivatives have reached their limits in fp32, and an infinite z gives no 0
+// times infinity.  (Its square is finite too.)
+constexpr float kFar = 1e18f;
+__device__ __forceinline__ float above(float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(-kFar));
+    return r;
+}
+__device__ __forceinline__ float below(float z) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(z), "f"(kFar));
+    return r;
+}
+
 // act(a), act(b) in place.  gelu: z P(z) = max(z, 0) - |z| T, T the upper tail at
-// |z| that normal_integral computes; |z| is held below 1e18, where T is 0, so
-// that an infinite z gives no 0 times infinity.
+// |z| that normal_integral computes.
 template <int ACT>
 __device__ __forceinline__ void act_pair(float &a, float &b) {
     if (ACT == CUDAIR_ACT_RELU) {
         a = relu(a);
         b = relu(b);
     } else if (ACT == CUDAIR_ACT_SILU) {
-        const Pair z = pair(a, b);
+        const Pair z = pair(above(a), above(b));
         const Pair e = exp2_fast2(mul2(z, pair(-kLog2E)));
         unpair(mul2(z, rcp_fast2(add2(e, pair(1.0f)))), a, b);
     } else if (ACT == CUDAIR_ACT_GELU_TANH) {
-        const Pair z = pair(a, b);
+        const Pair z = pair(above(a), above(b));
         const Pair y = fma2(mul2(z, z), pair(-kLog2E * kGeluC * kGeluB), pair(-kLog2E * kGeluC));
         unpair(mul2(z, rcp_fast2(add2(exp2_fast2(mul2(z, y)), pair(1.0f)))), a, b);
     } else if (ACT == CUDAIR_ACT_GELU) {
-        const Pair u = pair(fminf(fabsf(a), 1e18f), fminf(fabsf(b), 1e18f));
+        const Pair u = pair(fminf(fabsf(a), kFar), fminf(fabsf(b), kFar));
         const Pair E = exp2_fast2(mul2(mul2(u, pair(-0.5f * kLog2E)), u));
         const Pair t = rcp_fast2(fma2(u, pair(kTailQ), pair(1.0f)));
         Pair h = pair(kTail[6]);
@@ -163,19 +177,22 @@ __device__ __forceinline__ void act_both(float z, float &value, float &grad) {
         value = relu(z);
         grad = z <= 0.0f ? 0.0f : 1.0f;
     } else if (ACT == CUDAIR_ACT_SILU) {
+        z = above(z);
         const float s = sigmoid(z);
         value = z * s;
-        grad = s * (1.0f + z * (1.0f - s));
+        grad = s * (1.0f + below(z) * (1.0f - s));
     } else if (ACT == CUDAIR_ACT_GELU) {
         float P, E;
+        z = above(z);
         normal_integral(z, P, E);
         value = z * P;
-        grad = P + z * (0.3989422804014327f * E);
+        grad = P + below(z) * (0.3989422804014327f * E);
     } else if (ACT == CUDAIR_ACT_GELU_TANH) {
+        z = above(z);
         const float z2 = z * z;
         const float s = gelu_tanh_sigmoid(z, z2);
         value = z * s;
-        // s (1 - s) is zero where s is 0 or 1; z^2 may be infinite there.
+        // s (1 - s) is zero where s is 0 or 1; z^2 may be infinite there (z is not held from above).
         const float w = s - s * s;
         grad = w == 0.0f ? s : s + w * (z * fmaf(3.0f * kGeluB * kGeluC, z2, kGeluC));
     } else {

@@ -340,9 +340,11 @@ int cudair_reduce_f32(const float *in, float *out, int32_t n, void *stream);
  * integral P; CUDAIR_ACT_GELU_TANH is z (1 + tanh(sqrt(2/pi) (z + 0.044715
  * z^3))) / 2; CUDAIR_ACT_SILU is z / (1 + e^-z).  The derivative of RELU at 0
  * is 0.  The values are computed in fp32 and are off, before they are rounded
- * to their type, by at most 2^-20 of the value plus what an exponent x of 24 bits
+ * to their type, by at most 2^-19 of the value plus what an exponent x of 24 bits
  * loses in e^x: |x| 2^-21, x = z^2 / 2 (GELU), 2 sqrt(2/pi) (|z| + 0.044715 |z|^3)
- * (GELU_TANH), |z| (SILU); exponentials below 2^-126 count as 0. */
+ * (GELU_TANH), |z| (SILU); exponentials below 2^-126 count as 0.  At an
+ * infinite z values and derivatives are their limits (-0 counts as 0); a NaN
+ * stays one (RELU's derivative there is 1). */
 enum {
     CUDAIR_ACT_NONE = 0, CUDAIR_ACT_RELU = 1, CUDAIR_ACT_GELU = 2,
     CUDAIR_ACT_GELU_TANH = 3, CUDAIR_ACT_SILU = 4

@@ -92,3 +92,39 @@ def test_backward_values_keep_their_relative_accuracy(dev, cudair, act, dtype):
     kernels.gated_backward(one, x, w, w, g, one, dg, du, act=act)
     ratio = off(du[0], g[0].double(), act)
     assert ratio[0] <= 1, ratio
+
+
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("act", ACTS + ("relu", "none"))
+def test_infinite_and_far_arguments_reach_the_limits(dev, cudair, act, dtype, M):
+    """Values: 0 and z; derivatives: 0 and 1; a NaN stays one.  The same for the largest finite
+    arguments, in the forward's epilogue (z by the bias) and in the gradient's element-wise step."""
+    import torch
+    from cudair import kernels
+    dt, inf, nan = getattr(torch, dtype), float("inf"), float("nan")
+    far = float(torch.finfo(dt).max)
+    z = torch.tensor([-inf, -far, -far / 4, far / 4, far, inf, nan, -100], device=dev)
+    low = [0.0] * 3 if act != "none" else [-inf, -far, -far / 4]
+    want = torch.tensor(low + [far / 4, far, inf, nan, 0 if act != "none" else -100], device=dev)
+    slope = torch.tensor([0.0 if act != "none" else 1.0] * 3 + [1.0] * 3, device=dev)
+    same = lambda p, q: bool(((p == q) | (p.isnan() & q.isnan())).all())  # noqa: E731
+    d, zz = torch.empty(M, 8, device=dev), torch.empty(M, 8, dtype=dt, device=dev)
+    kernels.linear(torch.empty(M, 0, dtype=dt, device=dev), torch.empty(0, 8, dtype=dt, device=dev), d, bias=z,
+                   z=zz, act=act)
+    assert same(d, want.expand(M, 8)), d[0]
+    assert same(zz, z.to(dt).expand(M, 8)), zz[0]
+    # linear_backward: dZ = act'(Z); gated_backward: dG = act'(G), dU = act(G), with dH = U = 1.
+    ones = torch.ones_like(zz)
+    x, w = torch.empty(M, 0, dtype=dt, device=dev), torch.empty(0, 8, dtype=dt, device=dev)
+    dg, du, dz = (torch.empty_like(zz) for _ in range(3))
+    kernels.gated_backward(ones, x, w, w, zz, ones, dg, du, act=act)
+    assert same(du.float(), want.to(dt).float().expand(M, 8)), du[0]
+    grads = [dg]
+    if act != "none":
+        kernels.linear_backward(ones, x, w, z=zz, dz=dz, act=act)
+        grads.append(dz)
+    for g in grads:
+        assert torch.equal(g[:, :6].float(), slope.expand(M, 6)), g[0]
+        assert act == "none" or act == "relu" or bool(g[:, 6].isnan().all())
+    assert kernels.wait_status(clear=True) == 0
