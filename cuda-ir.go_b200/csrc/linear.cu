@@ -238,7 +238,7 @@ cudaError_t act_grad_start(const cudaLaunchConfig_t &cfg, const EwArgs &p, bool 
                 : cudaLaunchKernelEx(&cfg, act_grad_kernel<GATED, SUM, false, false>, p);
 }
 
-int act_grad_launch(EwArgs &p, bool gated, bool bf16, bool dy_f32, int sm_count, cudaStream_t stream) {
+int act_grad_launch(EwArgs &p, bool gated, bool bf16, bool dy_f32, int pdl_mode, int sm_count, cudaStream_t stream) {
     const int64_t strips = (static_cast<int64_t>(p.N) + EW_COLS - 1) / EW_COLS;
     const bool sum = p.dbias != nullptr;
     const int64_t step = EW_ROWS * 4;  // whole batches
@@ -275,8 +275,8 @@ int act_grad_launch(EwArgs &p, bool gated, bool bf16, bool dy_f32, int sm_count,
     cfg.gridDim = dim3(static_cast<unsigned>(strips * chunks), 1, 1);
     cfg.blockDim = dim3(EW_THREADS, 1, 1);
     cfg.stream = stream;
-    cfg.attrs = gemm_pdl_mode() > 0 ? attr : attr + 1;
-    cfg.numAttrs = (gemm_pdl_mode() > 0 ? 1 : 0) + (sum ? 1 : 0);
+    cfg.attrs = pdl_mode > 0 ? attr : attr + 1;
+    cfg.numAttrs = (pdl_mode > 0 ? 1 : 0) + (sum ? 1 : 0);
     const cudaError_t e = gated ? act_grad_start<true, false>(cfg, p, bf16, dy_f32)
                           : sum ? act_grad_start<false, true>(cfg, p, bf16, dy_f32)
                                 : act_grad_start<false, false>(cfg, p, bf16, dy_f32);
@@ -453,6 +453,7 @@ CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     if (q->residual == q->d && q->residual && q->ldres != q->ldd)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a residual in D's memory needs D's pitch", op);
     Product p;
+    p.pdl_mode = gemm_pdl_mode();
     p.jobs = 1;
     Job &j = p.job[0];
     j.M = q->M;
@@ -496,6 +497,7 @@ CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
     CUDAIR_TRY(check_distinct(op, "g", q->g, {x, wg, wu, q->u}));
     CUDAIR_TRY(check_distinct(op, "u", q->u, {x, wg, wu}));
     Product p;
+    p.pdl_mode = gemm_pdl_mode();
     p.jobs = 1;
     p.gated = true;
     Job &j = p.job[0];
@@ -567,6 +569,8 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
 
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
+    Product p;
+    p.pdl_mode = gemm_pdl_mode();
     // dZ, and the bias's gradient from it (M = 0: its empty sums).
     const bool elementwise = q->N > 0 && ((own_dz && q->M > 0) || q->dbias);
     if (elementwise) {
@@ -581,11 +585,10 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         e.ldz = q->ldz;
         e.lddz = q->lddz;
         e.dbias = q->dbias;
-        CUDAIR_TRY(act_grad_launch(e, false, bf16, dy_f32, sms, s));
+        CUDAIR_TRY(act_grad_launch(e, false, bf16, dy_f32, p.pdl_mode, sms, s));
     }
     const void *dz = own_dz ? q->dz : q->dy;
     const int64_t lddz = own_dz ? q->lddz : q->lddy;
-    Product p;
     p.bf16 = bf16;
     p.chained = elementwise;
     if (want_da) {
@@ -666,6 +669,8 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
     if (want_dw) CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->dwu}));  // M = 0 writes them too
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
+    Product p;
+    p.pdl_mode = gemm_pdl_mode();
     const bool elementwise = q->M > 0 && q->N > 0;
     if (elementwise) {
         EwArgs e = {};
@@ -682,9 +687,8 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         e.ldu = q->ldu;
         e.lddz = q->lddg;
         e.lddu = q->lddu;
-        CUDAIR_TRY(act_grad_launch(e, true, bf16, false, sms, s));
+        CUDAIR_TRY(act_grad_launch(e, true, bf16, false, p.pdl_mode, sms, s));
     }
-    Product p;
     p.bf16 = bf16;
     p.chained = elementwise;
     if (want_dx) {

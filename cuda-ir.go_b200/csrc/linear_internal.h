@@ -52,12 +52,15 @@ struct Product {
     // cudair_set_gemm_pdl.  It waits for that kernel before it reads what the
     // call computes.
     bool chained = false;
+    // That mode, read once by the entry point: another thread may set it while
+    // the call's kernels, which rely on one another's launches, are being set up.
+    int pdl_mode = 0;
 
-    bool pdl() const { return chained || gemm_pdl_mode() > 0; }
+    bool pdl() const { return chained || pdl_mode > 0; }
     // Whether weights may be requested before that wait: nothing that is still
     // running writes them.  A chained kernel's predecessors are the call's own,
     // unless the call's first kernel overlaps the caller's (mode 1).
-    bool weights_early() const { return gemm_pdl_mode() == 2 || (chained && gemm_pdl_mode() == 0); }
+    bool weights_early() const { return pdl_mode == 2 || (chained && pdl_mode == 0); }
     int tiles_of_b() const { return gated ? 2 : 1; }
 };
 

@@ -1,0 +1,60 @@
+"""What the entry points of the feed-forward operators launch, on CPU: the
+object file of linear.cu linked with fakes of the kernels below it and of the
+runtime's launch (linear_host/launches.cpp)."""
+import itertools
+import os
+import re
+import subprocess
+import sys
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+PKG = os.path.join(os.path.dirname(HERE), "cuda-ir.go_b200")
+
+
+@pytest.fixture(scope="module")
+def launches(tmp_path_factory):
+    """launches(call, modes) -> the lines the call's launches print."""
+    sys.path.insert(0, PKG)
+    import build
+    build.build(force=False, verbose=False)
+    exe = str(tmp_path_factory.mktemp("linear_host") / "launches")
+    # nvcc finds its own headers and runtime; the host compiler alone may not.
+    subprocess.run([build.NVCC, "-std=c++17", "-cudart", "shared", "-o", exe,
+                    os.path.join(HERE, "linear_host", "launches.cpp"),
+                    os.path.join(PKG, "_build", "linear.cu.o")], check=True, capture_output=True, text=True)
+
+    def run(call, modes):
+        r = subprocess.run([exe, call] + [str(m) for m in modes], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, (call, modes, r.returncode, r.stderr)
+        return [{k: int(v) for k, v in re.findall(r"(\w+)=(\d+)", line)} | {"kernel": line.split()[0]}
+                for line in r.stdout.splitlines()]
+    return run
+
+
+CALLS = {"linear": 1, "gated": 1, "linear_backward": 2, "gated_backward": 2}
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_launch_modes(launches, call):
+    """Weights are requested early only where nothing that may still run writes them: behind the
+    call's own element-wise kernel if that one waits for the stream, or if the caller says so."""
+    for mode in (0, 1, 2):
+        got = launches(call, [mode])
+        assert len(got) == CALLS[call]
+        product = got[-1]
+        assert product["kernel"] == "product"
+        assert product["programmatic"] == (1 if mode or len(got) == 2 else 0)
+        assert product["weights_early"] == (1 if mode == 2 or (mode == 0 and len(got) == 2) else 0)
+        if len(got) == 2:
+            assert got[0]["kernel"] == "elementwise" and got[0]["programmatic"] == (1 if mode else 0)
+            assert (got[0]["cluster"] > 0) == (call == "linear_backward")  # the bias's sums
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_a_mode_set_during_the_call_does_not_mix(launches, call):
+    """Whatever the mode reads as during a call, its launches are those of one mode."""
+    whole = [launches(call, [m]) for m in (0, 1, 2)]
+    for modes in itertools.product((0, 1, 2), repeat=4):
+        assert launches(call, modes) in whole, modes
