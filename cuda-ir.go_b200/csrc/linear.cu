@@ -14,6 +14,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <initializer_list>
 
 #include "cudair_internal.h"
@@ -343,6 +344,19 @@ int check_mat(const char *op, const char *name, const void *p, int64_t ld, int64
         if (rc_ != CUDAIR_OK) return rc_;       \
     } while (0)
 
+// cudair_set_linear_kernel: the kernel, and 16 bits further up the width.
+std::atomic<int> g_kernel{0};
+
+// A call's products, under the settings of the process as they are now.
+Product new_product() {
+    const int k = g_kernel.load();
+    Product p;
+    p.pdl_mode = gemm_pdl_mode();
+    p.kernel = k & 0xFFFF;
+    p.width = k >> 16;
+    return p;
+}
+
 Operand operand(const void *p, int64_t ld, bool mn) {
     Operand o;
     o.p = p;
@@ -362,6 +376,9 @@ OutMat out_mat(void *p, int64_t ld, bool f32) {
 
 namespace {
 
+// What cudair_set_linear_kernel may choose.
+constexpr int kSplit = 1, kPairs = 2;
+
 // One launch, by the kernel that is the faster one by their estimates.  Up to
 // 64 rows that is the split kernel: the pair kernel's 256-row tiles would read the
 // weights at the pace of few SMs (gated 1 x 4672 x 7296: 124 against 26 us).
@@ -371,14 +388,16 @@ struct Launch {
     double time = 0.0;
 };
 int plan_launch(const Product &p, int sm_count, Launch *l) {
-    CUDAIR_TRY(split_plan(p, &l->plan));
-    l->time = l->plan.time;
-    bool few = true;
-    for (int i = 0; i < p.jobs; ++i) few = few && p.job[i].M <= 64;
-    if (few) return CUDAIR_OK;
+    if (p.kernel != kPairs) {
+        CUDAIR_TRY(split_plan(p, &l->plan));
+        l->time = l->plan.time;
+        bool few = true;
+        for (int i = 0; i < p.jobs; ++i) few = few && p.job[i].M <= 64;
+        if (few || p.kernel == kSplit) return CUDAIR_OK;
+    }
     double pair = 0.0;
     CUDAIR_TRY(product_pair_time(p, sm_count, &pair));
-    if (pair < l->time) {
+    if (p.kernel == kPairs || pair < l->time) {
         l->split = false;
         l->time = pair;
     }
@@ -426,6 +445,22 @@ int product_launch(const Product &p, cudaStream_t stream) {
 using namespace cudair;
 using namespace cudair::ffn;
 
+CUDAIR_API int cudair_set_linear_kernel(int kernel, int width) {
+    clear_error();
+    if (kernel < 0 || kernel > 2)
+        return set_error(CUDAIR_ERR_INVALID,
+                         "cudair: linear kernel %d, want 0 (automatic), 1 (split) or 2 (CTA pairs)", kernel);
+    bool known = width == 0;
+    for (const int w : {192, 224, 256, 384, 448, 512}) known = known || (kernel == kPairs && width == w);
+    if (!known)
+        return set_error(CUDAIR_ERR_INVALID,
+                         "cudair: linear tile width %d, want 0 (automatic) or, of CTA pairs, 192, 224, 256, 384, 448 or "
+                         "512",
+                         width);
+    g_kernel.store(kernel | width << 16);
+    return CUDAIR_OK;
+}
+
 CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     clear_error();
     const char *op = "linear";
@@ -452,8 +487,7 @@ CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     CUDAIR_TRY(check_distinct(op, "z", q->z, {a, b, q->bias, q->residual}));
     if (q->residual == q->d && q->residual && q->ldres != q->ldd)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a residual in D's memory needs D's pitch", op);
-    Product p;
-    p.pdl_mode = gemm_pdl_mode();
+    Product p = new_product();
     p.jobs = 1;
     Job &j = p.job[0];
     j.M = q->M;
@@ -496,8 +530,9 @@ CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
     CUDAIR_TRY(check_distinct(op, "h", q->h, {x, wg, wu, q->g, q->u}));
     CUDAIR_TRY(check_distinct(op, "g", q->g, {x, wg, wu, q->u}));
     CUDAIR_TRY(check_distinct(op, "u", q->u, {x, wg, wu}));
-    Product p;
-    p.pdl_mode = gemm_pdl_mode();
+    Product p = new_product();
+    if (p.width == 224 || p.width == 448)  // blocks of 224 columns: 112 of each product, not whole chunks of 32
+        return set_error(CUDAIR_ERR_INVALID, "cudair: %s: tiles of %d columns do not take two weights", op, p.width);
     p.jobs = 1;
     p.gated = true;
     Job &j = p.job[0];
@@ -569,8 +604,7 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
 
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
-    Product p;
-    p.pdl_mode = gemm_pdl_mode();
+    Product p = new_product();
     // dZ, and the bias's gradient from it (M = 0: its empty sums).
     const bool elementwise = q->N > 0 && ((own_dz && q->M > 0) || q->dbias);
     if (elementwise) {
@@ -669,8 +703,7 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
     if (want_dw) CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->dwu}));  // M = 0 writes them too
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
-    Product p;
-    p.pdl_mode = gemm_pdl_mode();
+    Product p = new_product();
     const bool elementwise = q->M > 0 && q->N > 0;
     if (elementwise) {
         EwArgs e = {};

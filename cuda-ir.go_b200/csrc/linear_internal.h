@@ -55,6 +55,8 @@ struct Product {
     // That mode, read once by the entry point: another thread may set it while
     // the call's kernels, which rely on one another's launches, are being set up.
     int pdl_mode = 0;
+    // cudair_set_linear_kernel, read with it.
+    int kernel = 0, width = 0;
 
     bool pdl() const { return chained || pdl_mode > 0; }
     // Whether weights may be requested before that wait: nothing that is still

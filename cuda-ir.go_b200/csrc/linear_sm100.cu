@@ -736,6 +736,7 @@ Deal best_deal(const Product &p, int pairs, Width *width) {
     best.time = 1e300;
     for (const Width &w : kWidths) {
         if (p.gated && w.bn % 64) continue;  // its columns of D are half as many
+        if (p.width && p.width != w.bn * w.nb) continue;
         const Deal d = deal(p, w, pairs);
         if (d.time < best.time) {
             best = d;

@@ -49,6 +49,7 @@ SIGNATURES = {
     "cudair_linear_backward": (c_int, [c_vp, c_vp]),
     "cudair_gated": (c_int, [c_vp, c_vp]),
     "cudair_gated_backward": (c_int, [c_vp, c_vp]),
+    "cudair_set_linear_kernel": (c_int, [c_int, c_int]),
     "cudair_set_gemm_variant": (c_int, [c_int]),
     "cudair_set_gemm_pdl": (c_int, [c_int]),
     "cudair_vecadd": (c_int, [c_vp, c_vp, c_vp, ctypes.c_int32, c_vp]),

@@ -375,6 +375,13 @@ def set_gemm_pdl(mode: int) -> None:
     check(lib().cudair_set_gemm_pdl(mode))
 
 
+def set_linear_kernel(kernel: int, width: int = 0) -> None:
+    """The kernel of linear, gated and their gradients: 0 = automatic, 1 = split
+    kernel, 2 = CTA pairs with tiles of width 192, 224, 256, 384, 448 or 512
+    (gated: not 224 or 448) or, with 0, the automatic one."""
+    check(lib().cudair_set_linear_kernel(kernel, width))
+
+
 def vecadd(a, b, out, stream=None) -> None:
     """out = a + b over fp32 vectors (VecAdd's operands)."""
     import torch

@@ -450,6 +450,18 @@ typedef struct cudair_gated_backward_args {
 } cudair_gated_backward_args;
 int cudair_gated_backward(const cudair_gated_backward_args *args, void *stream);
 
+/*
+ * Selects the kernel that computes the products of the four calls above, for
+ * subsequent calls in this process: 0 = automatic (the faster one by an
+ * estimate for the sizes; the split kernel up to 64 rows), 1 = the split kernel
+ * (the contraction cut between the CTAs of a cluster), 2 = persistent CTA pairs
+ * with tiles of 256 rows.  width: with 2, the columns of a tile, 192, 224,
+ * 256, 384, 448 or 512 (shared by both products of cudair_gated, which refuses 224
+ * and 448), or 0 for the estimate's choice; else 0.  All choices compute the same result
+ * within fp32 rounding; the choice only affects speed.
+ */
+int cudair_set_linear_kernel(int kernel, int width);
+
 /* ---- seeded synthetic operands -------------------------------------------- */
 
 enum { CUDAIR_FILL_F32 = 0, CUDAIR_FILL_F16 = 1 };

@@ -1,11 +1,12 @@
 // The entry points of linear.cu over fakes of everything below them, so that
 // what one call launches can be read without a GPU.
 //
-//   launches CALL MODE [MODE...]
+//   launches CALL MODE [MODE...] [-- KERNEL WIDTH]
 //
 // CALL is linear, gated, linear_backward or gated_backward; the launch mode
 // (cudair_set_gemm_pdl) reads as the MODEs one after the other, the last one
-// from then on, as if another thread set it during the call.  Prints one line
+// from then on, as if another thread set it during the call.  KERNEL and WIDTH go
+// to cudair_set_linear_kernel first.  Prints one line
 // per launch: the element-wise kernel's attributes, and what a product launch
 // would do about its own.
 #include <cuda_runtime.h>
@@ -53,7 +54,10 @@ int product_pair_time(const Product &, int, double *us) {
     *us = 2.0;
     return CUDAIR_OK;
 }
-int product_pair_launch(const Product &, int, unsigned int *, cudaStream_t) { abort(); }
+int product_pair_launch(const Product &p, int, unsigned int *, cudaStream_t) {
+    printf("pairs jobs=%d programmatic=%d weights_early=%d width=%d\n", p.jobs, p.pdl(), p.weights_early(), p.width);
+    return CUDAIR_OK;
+}
 int product_split_launch(const Product &p, const SplitPlan &, unsigned int *, cudaStream_t) {
     printf("product jobs=%d programmatic=%d weights_early=%d\n", p.jobs, p.pdl(), p.weights_early());
     return CUDAIR_OK;
@@ -75,7 +79,9 @@ extern "C" cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *cfg, const 
 
 int main(int argc, char **argv) {
     if (argc < 3) return 2;
-    for (int i = 2; i < argc && g_mode_count < 16; ++i) g_modes[g_mode_count++] = atoi(argv[i]);
+    int i = 2;
+    for (; i < argc && strcmp(argv[i], "--") && g_mode_count < 16; ++i) g_modes[g_mode_count++] = atoi(argv[i]);
+    if (i + 2 < argc && cudair_set_linear_kernel(atoi(argv[i + 1]), atoi(argv[i + 2])) != CUDAIR_OK) return 3;
     const char *how = argv[1];
     // Sixteen separate arrays; nothing reads them.
     char *at[16];

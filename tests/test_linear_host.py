@@ -15,7 +15,7 @@ PKG = os.path.join(os.path.dirname(HERE), "cuda-ir.go_b200")
 
 @pytest.fixture(scope="module")
 def launches(tmp_path_factory):
-    """launches(call, modes) -> the lines the call's launches print."""
+    """launches(call, modes, kernel, width) -> what the call's launches print."""
     sys.path.insert(0, PKG)
     import build
     build.build(force=False, verbose=False)
@@ -25,8 +25,12 @@ def launches(tmp_path_factory):
                     os.path.join(HERE, "linear_host", "launches.cpp"),
                     os.path.join(PKG, "_build", "linear.cu.o")], check=True, capture_output=True, text=True)
 
-    def run(call, modes):
-        r = subprocess.run([exe, call] + [str(m) for m in modes], capture_output=True, text=True, timeout=60)
+    def run(call, modes, kernel=0, width=0, refused=None):
+        r = subprocess.run([exe, call] + [str(m) for m in modes] + ["--", str(kernel), str(width)],
+                           capture_output=True, text=True, timeout=60)
+        if refused:
+            assert r.returncode == 1 and re.search(refused, r.stderr), (r.returncode, r.stderr)
+            return []
         assert r.returncode == 0, (call, modes, r.returncode, r.stderr)
         return [{k: int(v) for k, v in re.findall(r"(\w+)=(\d+)", line)} | {"kernel": line.split()[0]}
                 for line in r.stdout.splitlines()]
@@ -58,3 +62,23 @@ def test_a_mode_set_during_the_call_does_not_mix(launches, call):
     whole = [launches(call, [m]) for m in (0, 1, 2)]
     for modes in itertools.product((0, 1, 2), repeat=4):
         assert launches(call, modes) in whole, modes
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_the_kernel_may_be_chosen(launches, call):
+    assert launches(call, [0], 1)[-1]["kernel"] == "product"  # the split kernel
+    for width in (0, 192, 224, 256, 384, 448, 512):
+        if call == "gated" and width in (224, 448):
+            launches(call, [0], 2, width, refused="gated: tiles of %d columns do not take two weights" % width)
+        else:
+            got = launches(call, [0], 2, width)[-1]
+            assert got["kernel"] == "pairs" and got["width"] == width
+
+
+def test_kernel_choices_that_are_refused(cudair):
+    from cudair import _lib, kernels
+    for kernel, width, message in ((-1, 0, "linear kernel -1"), (3, 0, "linear kernel 3"), (2, 128, "tile width 128"),
+                                   (2, -256, "tile width -256"), (1, 256, "tile width 256"), (0, 512, "tile width 512")):
+        with pytest.raises(_lib.CudairError, match=message):
+            kernels.set_linear_kernel(kernel, width)
+    kernels.set_linear_kernel(0)
