@@ -160,8 +160,10 @@ __global__ void __launch_bounds__(EW_THREADS, (EwCfg<GATED, f32>::BLOCKS)) act_g
         }
     };
 
-    if (threadIdx.x == 0) grid_launch_dependents();  // the products may set up
     grid_dependency_wait();
+    // The products may set up, and request weights: after the wait, so that all
+    // kernels before this one have ended.
+    if (threadIdx.x == 0) grid_launch_dependents();
     if (col < p.N) {
         const bool whole = col + 8 <= p.N;
         long long r0 = first + ty;

@@ -310,7 +310,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     cluster_sync();  // barriers of both CTAs initialised before any remote arrive
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
-    if (threadIdx.x == 0) grid_launch_dependents();  // cudair_set_gemm_pdl
 
     auto give_up = [&]() { st_shared_cluster_u32(peer_abort, 1u); };
 
@@ -318,6 +317,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         // ---------------- TMA producers (both CTAs): A, B ----------------
         if (lane == 0) {
             grid_dependency_wait();
+            // Only now may the next kernel of the stream start (cudair_set_gemm_pdl):
+            // then all before this one have ended, and that kernel may request
+            // weights that this one does not write before it waits for this one.
+            if (warp == 0) grid_launch_dependents();
             const uint64_t policy = l2_policy_evict_normal();
             uint32_t stage = 0, phase = 0;
             bool ok = true;

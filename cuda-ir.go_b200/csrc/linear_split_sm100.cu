@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(threads(EPI_WARPS), 2)
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
     // cudair_set_gemm_pdl: only now, with its columns in hand, so that no CTA of
-    // the next kernel takes them and waits for this one.
+    // the next kernel takes them and waits for this one; and past the producer's wait
+    // for the preceding kernel (the barrier above), so that all before have ended.
     if (threadIdx.x == 64) grid_launch_dependents();
 
     if (warp == 0) {

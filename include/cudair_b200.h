@@ -227,9 +227,13 @@ int cudair_set_gemm_variant(int variant);
  * it reads A, B, C or its workspace.  mode 2: as 1, and the few-row kernel
  * requests the first stages of B before the wait (the square-tile kernels
  * treat it as 1).  The caller promises that the preceding kernel does not
- * write B (weights).  Results are identical in all modes.  Applies to
+ * write B (weights), and where GEMMs run back to back, that none of them does:
+ * a GEMM may let its successor start before its own predecessor has ended.  (The
+ * feed-forward calls below do not: each lets the next kernel start once all before it have
+ * ended.)  Results are identical in all modes.  Applies to
  * subsequent GEMM calls (cudair_gemm_f16f32, cudair_gemm, cudair_matmul16
- * above n = 512) in this process.
+ * above n = 512) and to the feed-forward calls, whose few-row kernel requests weights
+ * early in mode 2, in this process.
  */
 int cudair_set_gemm_pdl(int mode);
 

@@ -103,3 +103,58 @@ def test_calls_repeat_exactly(dev, cudair, kernel):
             for o in outs:
                 assert all(torch.equal(t, v) for t, v in zip(o, want)), turn
     assert kernels.wait_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("mode", [1, 2])
+@pytest.mark.parametrize("last", ["linear", "linear_backward", "gated_backward"])
+def test_weights_written_two_kernels_before(dev, cudair, mode, last):
+    """A long kernel writes a matrix, a short one that needs nothing of it follows, and the third call's
+    weights are that matrix: programmatic launches must not let the third read it before it is there.
+    (Launch mode 2 lets a caller rule out the preceding kernel only.)"""
+    import torch
+    from cudair import kernels
+    bf = torch.bfloat16
+    n, K = 256, 1 << 18  # one tile, 4096 k-blocks: about a millisecond on two SMs
+    a, b = (torch.randn(n, K, device=dev).to(bf) for _ in range(2))
+    t, y = (torch.empty(n, n, dtype=bf, device=dev) for _ in range(2))
+    s = torch.randn(n, n, device=dev).to(bf)
+    one = torch.randn(8, n, device=dev).to(bf)
+    z, dz, dg, du = (torch.randn(8, n, device=dev).to(bf) for _ in range(4))
+    got = torch.empty(8, n, device=dev)
+
+    def writer():
+        kernels.set_linear_kernel(PAIRS, 256)
+        kernels.linear(a, b, t, act="silu", b_trans=True)
+
+    def between():
+        kernels.linear(s, s, y)
+
+    def reader():
+        kernels.set_linear_kernel(SPLIT)
+        if last == "linear":
+            kernels.linear(one, t, got)
+        elif last == "linear_backward":
+            kernels.linear_backward(one, one, t, z=z, dz=dz, da=got, act="silu")
+        else:
+            kernels.gated_backward(one, one, t, t, z, z, dg, du, dx=got)
+
+    try:
+        writer()
+        torch.cuda.synchronize()
+        reader()
+        torch.cuda.synchronize()
+        want = got.clone()
+        kernels.set_gemm_pdl(mode)
+        for _ in range(10):
+            t.fill_(11.0)
+            got.fill_(0.0)
+            torch.cuda.synchronize()
+            writer()
+            between()
+            reader()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+    finally:
+        kernels.set_gemm_pdl(0)
+        kernels.set_linear_kernel(0)
+    assert kernels.wait_status(clear=True) == 0
