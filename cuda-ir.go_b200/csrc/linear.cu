@@ -299,13 +299,14 @@ int check_sizes(const char *op, int64_t M, int64_t N, int64_t K) {
     return CUDAIR_OK;
 }
 
-// A contraction's length is bounded so that one tile's k-blocks take well under the
-// two seconds after which a device wait gives up.
+// What one accumulator sums is bounded so that a tile's k-blocks take well under the
+// two seconds after which a device wait gives up: 2^20 k-blocks of 0.73 us (tiles of
+// two blocks, the slowest) are 0.77 s.  `parts` contractions go into one accumulator.
 constexpr int64_t kMaxDepth = int64_t{1} << 26;
-int check_depth(const char *op, int64_t depth) {
-    if (depth > kMaxDepth)
+int check_depth(const char *op, int64_t depth, int parts = 1) {
+    if (depth > kMaxDepth / parts)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a contraction over %lld is too long (at most %lld)", op,
-                         (long long)depth, (long long)kMaxDepth);
+                         (long long)depth, (long long)(kMaxDepth / parts));
     return CUDAIR_OK;
 }
 
@@ -693,7 +694,7 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
         CUDAIR_TRY(check_mat(op, "dwu", q->dwu, q->lddwu, wcols, dw_f32 ? 4 : 2));
         if (q->M > 0) CUDAIR_TRY(check_mat(op, "x", q->x, q->ldx, q->K, 2));
     }
-    if (want_dx) CUDAIR_TRY(check_depth(op, q->N));
+    if (want_dx) CUDAIR_TRY(check_depth(op, q->N, 2));
     if (want_dw) CUDAIR_TRY(check_depth(op, q->M));
     if (q->M > 0 && q->N > 0 && q->K > 0) {
         CUDAIR_TRY(check_distinct(op, "dg", q->dg, {q->x, q->wg, q->wu, q->dx, q->dwg, q->dwu}));

@@ -442,7 +442,8 @@ int cudair_gated(const cudair_gated_args *args, void *stream);
  *   dX  = dG . Wg^T + dU . Wu^T                (M x K; fp32 with _DA_F32)
  *   dWg = X^T . dG,  dWu = X^T . dU            (as the weights; fp32 with _DB_F32)
  * dg and du are needed, and may be g's and u's (or dH's) own memory (same
- * pitch).  dx may be NULL; dwg and dwu are both given or both NULL.  Other
+ * pitch).  dx may be NULL; dwg and dwu are both given or both NULL.  N is at most
+ * 2^25 for dX, whose sums run over two contractions.  Other
  * rules as cudair_linear_backward.
  */
 typedef struct cudair_gated_backward_args {

@@ -82,3 +82,21 @@ def test_kernel_choices_that_are_refused(cudair):
         with pytest.raises(_lib.CudairError, match=message):
             kernels.set_linear_kernel(kernel, width)
     kernels.set_linear_kernel(0)
+
+
+def test_depth_counts_both_contractions_of_dx(cudair):
+    """dX = dG.Wg^T + dU.Wu^T is one sum over 2 N products."""
+    import ctypes
+
+    from cudair import _lib
+    P = 0x7F0000000000
+    n = 2 ** 25 + 8
+    at = [P + (i << 40) for i in range(9)]
+    args = dict(dh=at[0], x=None, wg=at[1], wu=at[2], g=at[3], u=at[4], dg=at[5], du=at[6], dx=at[7], M=4, N=n, K=16,
+                lddh=n, ldwg=n, ldwu=n, ldg=n, ldu=n, lddg=n, lddu=n, lddx=16, act=4)
+    assert cudair.lib().cudair_gated_backward(ctypes.byref(_lib.GatedBackwardArgs(**args)), None) == _lib.ERR_INVALID
+    assert "contraction over 33554440 is too long (at most 33554432)" in cudair.last_error()
+    # Without dX nothing sums over N: the next rule refuses this one.
+    args.update(dx=None, x=at[5], ldx=16)
+    assert cudair.lib().cudair_gated_backward(ctypes.byref(_lib.GatedBackwardArgs(**args)), None) == _lib.ERR_INVALID
+    assert "dg lies over another matrix" in cudair.last_error()
