@@ -154,6 +154,23 @@ def _dims(op, x, xname, w, wname, b_trans):
     return x.shape[0], w.shape[0 if b_trans else 1], x.shape[1]
 
 
+def _grad_dims(op, dy, yname, x, w, dx, dw, b_trans):
+    """(M, N, K) of a gradient's call: M x N from the upstream gradient, K from the
+    first of x, w, dx and dw that is given (0: none, and no product to compute)."""
+    for t, name in ((dy, yname), (x, "the input"), (w, "the weight"), (dx, "the input's gradient"),
+                    (dw, "the weight's gradient")):
+        if (t is not None or t is dy) and getattr(t, "ndim", 0) != 2:
+            raise CudairError(1, f"cudair: {op}: {name} must be a matrix")
+    for t, dim in ((x, 1), (w, 1 if b_trans else 0), (dx, 1), (dw, 1 if b_trans else 0)):
+        if t is not None:
+            return dy.shape[0], dy.shape[1], t.shape[dim]
+    return dy.shape[0], dy.shape[1], 0
+
+
+def _optional(op, name, t, dtypes, rows, cols, device):
+    return (None, 0) if t is None else _mat(op, name, t, dtypes, rows, cols, device)
+
+
 def linear(a, b, d, bias=None, residual=None, z=None, act="none", b_trans=False, stream=None) -> None:
     """d = act(a @ B + bias) + residual with B = b (K x N), or b.T when b_trans
     (b is N x K): one kernel (cudair_linear).  a and b are both fp16 or both
@@ -195,19 +212,21 @@ def linear_backward(dy, a, b, z=None, dz=None, da=None, db=None, dbias=None, act
     a's type or fp32 (the gradient of d, and so the residual's).  z (as linear
     stored it) is needed with an activation; dz (M x N of a's type) with an
     activation or an fp32 dy, and only then; it may be z's or dy's memory.
-    da and db are of a's type or fp32."""
+    da and db are of a's type or fp32.  a may be None without db (a frozen
+    weight), b without da."""
     import torch
     op, dev = "linear_backward", _device()
-    dt = _type(op, a, "a")
-    M, N, K = _dims(op, a, "a", b, "b", b_trans)
+    typed, name = next(((t, n) for t, n in ((a, "a"), (b, "b"), (dz, "dz"), (z, "z")) if t is not None), (dy, "dy"))
+    dt = _type(op, typed, name)
+    M, N, K = _grad_dims(op, dy, "dy", a, b, da, db, b_trans)
     t16, either = (dt,), (dt, torch.float32)
     w = (N, K) if b_trans else (K, N)
     flags = (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
     pdy, lddy = _mat(op, "dy", dy, either, M, N, dev)
     if dy.dtype is torch.float32:
         flags |= LINEAR_D_F32
-    pa, lda = _mat(op, "a", a, t16, M, K, dev)
-    pb, ldb = _mat(op, "b", b, t16, *w, dev)
+    pa, lda = _optional(op, "a", a, t16, M, K, dev)
+    pb, ldb = _optional(op, "b", b, t16, *w, dev)
     pz = pdz = pda = pdb = pdbias = None
     ldz = lddz = ldda = lddb = 0
     if z is not None:
@@ -258,18 +277,19 @@ def gated_backward(dh, x, wg, wu, g, u, dg, du, dx=None, dwg=None, dwu=None, act
     and du = dh * act(g) (M x N; they may be g's and u's memory), then, where
     given, dx = dg @ Wg.T + du @ Wu.T and dwg = x.T @ dg, dwu = x.T @ du
     (stored as the weights are; both or neither).  dx and the weights'
-    gradients are of x's type or fp32."""
+    gradients are of dh's type or fp32.  x may be None without dwg and dwu
+    (frozen weights), wg and wu without dx."""
     import torch
     op, dev = "gated_backward", _device()
-    dt = _type(op, x, "x")
-    M, N, K = _dims(op, x, "x", wg, "wg", b_trans)
+    dt = _type(op, dh, "dh")
+    M, N, K = _grad_dims(op, dh, "dh", x, wg, dx, dwg, b_trans)
     t16, either = (dt,), (dt, torch.float32)
     w = (N, K) if b_trans else (K, N)
     flags = (GEMM_BF16 if dt is torch.bfloat16 else 0) | (GEMM_B_T if b_trans else 0)
     pdh, lddh = _mat(op, "dh", dh, t16, M, N, dev)
-    px, ldx = _mat(op, "x", x, t16, M, K, dev)
-    pwg, ldwg = _mat(op, "wg", wg, t16, *w, dev)
-    pwu, ldwu = _mat(op, "wu", wu, t16, *w, dev)
+    px, ldx = _optional(op, "x", x, t16, M, K, dev)
+    pwg, ldwg = _optional(op, "wg", wg, t16, *w, dev)
+    pwu, ldwu = _optional(op, "wu", wu, t16, *w, dev)
     pg, ldg = _mat(op, "g", g, t16, M, N, dev)
     pu, ldu = _mat(op, "u", u, t16, M, N, dev)
     pdg, lddg = _mat(op, "dg", dg, t16, M, N, dev)
