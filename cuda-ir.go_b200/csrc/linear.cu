@@ -310,11 +310,61 @@ int check_depth(const char *op, int64_t depth, int parts = 1) {
     return CUDAIR_OK;
 }
 
-// An output in the place of an input or of another output.
-int check_distinct(const char *op, const char *name, const void *out, std::initializer_list<const void *> others) {
-    for (const void *o : others)
-        if (out && out == o)
+// Where a matrix lies, in bytes; no rows: nowhere.  (An operand that is given but not needed may
+// have no pitch: its first row counts.)
+struct Extent {
+    int64_t at = 0, pitch = 0, row = 0, rows = 0;
+};
+Extent extent(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
+    Extent e;
+    if (!p || rows == 0 || cols == 0) return e;
+    e.at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
+    e.pitch = ld * elem;
+    e.row = cols * elem;
+    e.rows = ld < cols ? 1 : rows;
+    return e;
+}
+
+// Whether two matrices of one pitch have a byte in common: rows i of a and j of b
+// do if (i - j) pitch lies strictly between d - a.row and d + b.row, d = b.at - a.at.  (Views of
+// one array, such as halves of its columns, interleave without that.)
+bool rows_meet(const Extent &a, const Extent &b, int64_t pitch) {
+    const int64_t d = b.at - a.at, low = d - a.row;
+    int64_t k = low / pitch - (low % pitch < 0 ? 1 : 0) + 1;  // the least that is above low / pitch
+    if (k < 1 - b.rows) k = 1 - b.rows;
+    return k < a.rows && k * pitch < d + b.row;
+}
+bool overlap(const Extent &a, const Extent &b) {
+    if (a.rows == 0 || b.rows == 0) return false;
+    if (a.at + (a.rows - 1) * a.pitch + a.row <= b.at || b.at + (b.rows - 1) * b.pitch + b.row <= a.at) return false;
+    if (a.rows == 1 || b.rows == 1 || a.pitch == b.pitch) {
+        const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+        return rows_meet(a, b, pitch > 0 ? pitch : 1);
+    }
+    const Extent &few = a.rows < b.rows ? a : b, &many = a.rows < b.rows ? b : a;
+    for (int64_t i = 0; i < few.rows; ++i) {
+        Extent one = few;
+        one.at += i * few.pitch;
+        one.rows = 1;
+        if (rows_meet(many, one, many.pitch)) return true;
+    }
+    return false;
+}
+
+// An output over an input or another output.
+int check_distinct(const char *op, const char *name, const Extent &out, std::initializer_list<Extent> others) {
+    for (const Extent &o : others)
+        if (overlap(out, o))
             return set_error(CUDAIR_ERR_INVALID, "cudair: %s: %s lies over another matrix of the call", op, name);
+    return CUDAIR_OK;
+}
+// An output that may be an input's own memory, element over element, but not else over it.
+int check_in_place(const char *op, const char *name, const Extent &out, std::initializer_list<Extent> inputs) {
+    for (const Extent &o : inputs)
+        if (out.at != o.at) {
+            const int rc = check_distinct(op, name, out, {o});
+            if (rc != CUDAIR_OK) return rc;
+        }
     return CUDAIR_OK;
 }
 
@@ -485,11 +535,15 @@ CUDAIR_API int cudair_linear(const cudair_linear_args *q, void *stream) {
     if (q->bias && (reinterpret_cast<uintptr_t>(q->bias) & (bias16 ? 1u : 3u)))
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: bias must be aligned to its elements", op);
     CUDAIR_TRY(check_depth(op, q->K));
-    const void *a = q->K > 0 ? q->a : nullptr, *b = q->K > 0 ? q->b : nullptr;
-    CUDAIR_TRY(check_distinct(op, "d", q->d, {a, b, q->bias, q->z}));
-    CUDAIR_TRY(check_distinct(op, "z", q->z, {a, b, q->bias, q->residual}));
+    const int d_size = d_f32 ? 4 : 2;
+    const Extent a = extent(q->a, q->lda, q->M, q->K, 2), b = extent(q->b, q->ldb, bt ? q->N : q->K, bt ? q->K : q->N, 2);
+    const Extent bias = extent(q->bias, q->N, 1, q->N, bias16 ? 2 : 4), z = extent(q->z, q->ldz, q->M, q->N, 2);
+    const Extent d = extent(q->d, q->ldd, q->M, q->N, d_size), res = extent(q->residual, q->ldres, q->M, q->N, d_size);
+    CUDAIR_TRY(check_distinct(op, "d", d, {a, b, bias, z}));
+    CUDAIR_TRY(check_distinct(op, "z", z, {a, b, bias, res}));
     if (q->residual == q->d && q->residual && q->ldres != q->ldd)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: a residual in D's memory needs D's pitch", op);
+    CUDAIR_TRY(check_in_place(op, "d", d, {res}));
     Product p = new_product();
     p.jobs = 1;
     Job &j = p.job[0];
@@ -529,10 +583,13 @@ CUDAIR_API int cudair_gated(const cudair_gated_args *q, void *stream) {
         CUDAIR_TRY(check_mat(op, "u", q->u, q->ldu, q->N, 2));
     }
     CUDAIR_TRY(check_depth(op, q->K));
-    const void *x = q->K > 0 ? q->x : nullptr, *wg = q->K > 0 ? q->wg : nullptr, *wu = q->K > 0 ? q->wu : nullptr;
-    CUDAIR_TRY(check_distinct(op, "h", q->h, {x, wg, wu, q->g, q->u}));
-    CUDAIR_TRY(check_distinct(op, "g", q->g, {x, wg, wu, q->u}));
-    CUDAIR_TRY(check_distinct(op, "u", q->u, {x, wg, wu}));
+    const int64_t wrows = bt ? q->N : q->K, wcols = bt ? q->K : q->N;
+    const Extent x = extent(q->x, q->ldx, q->M, q->K, 2), h = extent(q->h, q->ldh, q->M, q->N, 2);
+    const Extent wg = extent(q->wg, q->ldwg, wrows, wcols, 2), wu = extent(q->wu, q->ldwu, wrows, wcols, 2);
+    const Extent g = extent(q->g, q->ldg, q->M, q->N, 2), u = extent(q->u, q->ldu, q->M, q->N, 2);
+    CUDAIR_TRY(check_distinct(op, "h", h, {x, wg, wu, g, u}));
+    CUDAIR_TRY(check_distinct(op, "g", g, {x, wg, wu, u}));
+    CUDAIR_TRY(check_distinct(op, "u", u, {x, wg, wu}));
     Product p = new_product();
     if (p.width == 224 || p.width == 448)  // blocks of 224 columns: 112 of each product, not whole chunks of 32
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: tiles of %d columns do not take two weights", op, p.width);
@@ -595,15 +652,20 @@ CUDAIR_API int cudair_linear_backward(const cudair_linear_backward_args *q, void
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dbias must be 4-byte aligned", op);
     if (want_da) CUDAIR_TRY(check_depth(op, q->N));
     if (want_db) CUDAIR_TRY(check_depth(op, q->M));
-    if (q->M > 0 && q->N > 0 && q->K > 0) {
-        CUDAIR_TRY(check_distinct(op, "dz", q->dz, {q->a, q->b, q->da, q->db, q->dbias}));
-        CUDAIR_TRY(check_distinct(op, "da", q->da, {q->a, q->b, q->dy, q->z, q->db, q->dbias}));
-        CUDAIR_TRY(check_distinct(op, "db", q->db, {q->a, q->b, q->dy, q->z, q->dbias}));
-        CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->a, q->b, q->dy, q->z}));
-    }
-    // Outputs that a call with an empty dimension still writes.
-    if (q->M > 0 && q->N > 0) CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->dz, q->dy, q->z}));
-    if (want_db) CUDAIR_TRY(check_distinct(op, "dbias", q->dbias, {q->db}));
+    const int64_t wrows = bt ? q->N : q->K, wcols = bt ? q->K : q->N;
+    const Extent dy = extent(q->dy, q->lddy, q->M, q->N, dy_f32 ? 4 : 2);
+    const Extent z = extent(q->z, q->ldz, q->M, q->N, 2);
+    const Extent a = extent(q->a, q->lda, q->M, q->K, 2);
+    const Extent b = extent(q->b, q->ldb, wrows, wcols, 2);
+    const Extent edz = extent(q->dz, q->lddz, q->M, q->N, 2);
+    const Extent da = extent(want_da ? q->da : nullptr, q->ldda, q->M, q->K, da_f32 ? 4 : 2);
+    const Extent db = extent(want_db ? q->db : nullptr, q->lddb, wrows, wcols, db_f32 ? 4 : 2);
+    const Extent dbias = extent(q->dbias, q->N, 1, q->N, 4);
+    CUDAIR_TRY(check_in_place(op, "dz", edz, {dy, z}));
+    CUDAIR_TRY(check_distinct(op, "dz", edz, {a, b, da, db}));
+    CUDAIR_TRY(check_distinct(op, "da", da, {a, b, dy, z, db}));
+    CUDAIR_TRY(check_distinct(op, "db", db, {a, b, dy, z}));
+    CUDAIR_TRY(check_distinct(op, "dbias", dbias, {a, b, dy, z, edz, da, db}));
 
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
@@ -696,14 +758,24 @@ CUDAIR_API int cudair_gated_backward(const cudair_gated_backward_args *q, void *
     }
     if (want_dx) CUDAIR_TRY(check_depth(op, q->N, 2));
     if (want_dw) CUDAIR_TRY(check_depth(op, q->M));
-    if (q->M > 0 && q->N > 0 && q->K > 0) {
-        CUDAIR_TRY(check_distinct(op, "dg", q->dg, {q->x, q->wg, q->wu, q->dx, q->dwg, q->dwu}));
-        CUDAIR_TRY(check_distinct(op, "du", q->du, {q->x, q->wg, q->wu, q->dx, q->dwg, q->dwu}));
-        CUDAIR_TRY(check_distinct(op, "dx", q->dx, {q->x, q->wg, q->wu, q->dh, q->g, q->u, q->dwg, q->dwu}));
-        CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->x, q->wg, q->wu, q->dh, q->g, q->u, q->dwu}));
-        CUDAIR_TRY(check_distinct(op, "dwu", q->dwu, {q->x, q->wg, q->wu, q->dh, q->g, q->u}));
-    }
-    if (want_dw) CUDAIR_TRY(check_distinct(op, "dwg", q->dwg, {q->dwu}));  // M = 0 writes them too
+    const int64_t wrows = bt ? q->N : q->K;
+    const Extent dh = extent(q->dh, q->lddh, q->M, q->N, 2), g = extent(q->g, q->ldg, q->M, q->N, 2);
+    const Extent u = extent(q->u, q->ldu, q->M, q->N, 2), dg = extent(q->dg, q->lddg, q->M, q->N, 2);
+    const Extent du = extent(q->du, q->lddu, q->M, q->N, 2);
+    const Extent x = extent(q->x, q->ldx, q->M, q->K, 2);
+    const Extent wg = extent(q->wg, q->ldwg, wrows, wcols, 2);
+    const Extent wu = extent(q->wu, q->ldwu, wrows, wcols, 2);
+    const Extent dx = extent(want_dx ? q->dx : nullptr, q->lddx, q->M, q->K, dx_f32 ? 4 : 2);
+    const Extent dwg = extent(want_dw ? q->dwg : nullptr, q->lddwg, wrows, wcols, dw_f32 ? 4 : 2);
+    const Extent dwu = extent(want_dw ? q->dwu : nullptr, q->lddwu, wrows, wcols, dw_f32 ? 4 : 2);
+    if (overlap(dg, du)) return set_error(CUDAIR_ERR_INVALID, "cudair: %s: dg and du share memory", op);
+    CUDAIR_TRY(check_in_place(op, "dg", dg, {dh, g, u}));
+    CUDAIR_TRY(check_in_place(op, "du", du, {dh, g, u}));
+    CUDAIR_TRY(check_distinct(op, "dg", dg, {x, wg, wu, dx, dwg, dwu}));
+    CUDAIR_TRY(check_distinct(op, "du", du, {x, wg, wu, dx, dwg, dwu}));
+    CUDAIR_TRY(check_distinct(op, "dx", dx, {x, wg, wu, dh, g, u, dwg, dwu}));
+    CUDAIR_TRY(check_distinct(op, "dwg", dwg, {x, wg, wu, dh, g, u, dwu}));
+    CUDAIR_TRY(check_distinct(op, "dwu", dwu, {x, wg, wu, dh, g, u}));
     int sms = 0;
     CUDAIR_TRY(sm_count_current_device(&sms));  // the device and context checks
     Product p = new_product();

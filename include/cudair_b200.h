@@ -375,7 +375,8 @@ enum {
  *   z          M x N of A's type: Z as the backward pass reads it.
  * Every matrix is row-major with a 16-byte aligned base and a pitch of
  * whole 16 bytes; pitches are in elements.  No other output may overlap an
- * input or another output.  M or N of 0 is a no-op; K of 0 gives act(bias) +
+ * input or another output: that is refused (columns of one array beside one
+ * another do not overlap).  M or N of 0 is a no-op; K of 0 gives act(bias) +
  * residual (A and B are not read); K is at most 2^26.  A row of A that holds a
  * NaN or an infinity reaches its row of D only, a column of B its column.
  * Needs no workspace, so calls may overlap on several streams and in several

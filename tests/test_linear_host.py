@@ -100,3 +100,103 @@ def test_depth_counts_both_contractions_of_dx(cudair):
     args.update(dx=None, x=at[5], ldx=16)
     assert cudair.lib().cudair_gated_backward(ctypes.byref(_lib.GatedBackwardArgs(**args)), None) == _lib.ERR_INVALID
     assert "dg lies over another matrix" in cudair.last_error()
+
+
+# An output over part of another matrix of the call.  32 x 32 operands of 16 bits with a pitch of 64, so
+# that the 32 other columns of a row are another matrix's; `at` and `ld` place one of them.
+def _square(call, **over):
+    from cudair import _lib
+    P, n = 0x7F0000000000, 32
+    names = {"cudair_linear": (_lib.LinearArgs, "a b residual d z", "bias"),
+             "cudair_linear_backward": (_lib.LinearBackwardArgs, "dy a b z dz da db", "dbias"),
+             "cudair_gated": (_lib.GatedArgs, "x wg wu h g u", None),
+             "cudair_gated_backward": (_lib.GatedBackwardArgs, "dh x wg wu g u dg du dx dwg dwu", None)}[call]
+    cls, mats, vector = names
+    args = dict(M=n, N=n, K=n, act=4)
+    for i, m in enumerate(mats.split()):
+        args[m], args["ld" + {"residual": "res"}.get(m, m)] = P + (i << 20), 64
+    if vector:
+        args[vector] = P + (100 << 20)
+    args.update(over)
+    return cls(**args)
+
+
+def _refused(cudair, call, **over):
+    import ctypes
+
+    from cudair import _lib
+    args = _square(call, **over)
+    rc = getattr(cudair.lib(), call)(ctypes.byref(args), None)
+    assert rc == _lib.ERR_INVALID, (rc, cudair.last_error())
+    return cudair.last_error()
+
+
+AT = 0x7F0000000000
+PARTIAL = [  # call, output, what it lies over, that one's place in the order of _square
+    ("cudair_linear", "d", "a", 0), ("cudair_linear", "d", "b", 1), ("cudair_linear", "d", "residual", 2),
+    ("cudair_linear", "z", "d", 3), ("cudair_linear", "z", "residual", 2),
+    ("cudair_gated", "h", "x", 0), ("cudair_gated", "g", "wu", 2), ("cudair_gated", "u", "g", 4),
+    ("cudair_linear_backward", "dz", "dy", 0), ("cudair_linear_backward", "dz", "z", 3),
+    ("cudair_linear_backward", "da", "a", 1), ("cudair_linear_backward", "db", "da", 5),
+    ("cudair_gated_backward", "dg", "g", 4), ("cudair_gated_backward", "du", "dh", 0),
+    ("cudair_gated_backward", "du", "dg", 6), ("cudair_gated_backward", "dx", "u", 5),
+    ("cudair_gated_backward", "dwu", "dwg", 9)]
+
+
+@pytest.mark.parametrize("call,out,other,place", PARTIAL)
+def test_partial_overlaps_are_refused(cudair, call, out, other, place):
+    base = AT + (place << 20)
+    for shift in (16, 48, 128, 31 * 128 + 48, -16, -48, -31 * 128):
+        assert re.search("lies over another matrix|share memory", _refused(cudair, call, **{out: base + shift})), shift
+    # Another pitch: rows of 80 elements run into the other's columns.
+    assert re.search("lies over another matrix|share memory|pitch",
+                     _refused(cudair, call, **{out: base - 64, "ld" + out: 80}))
+
+
+def test_vectors_that_overlap_are_refused(cudair):
+    for at in (AT + (3 << 20) + 60, AT + (3 << 20) - 64, AT + (3 << 20) + 31 * 128 + 60):
+        assert "d lies over another" in _refused(cudair, "cudair_linear", bias=at)
+    for place in (0, 1, 2, 3, 4, 5, 6):
+        assert "dbias lies over another" in _refused(cudair, "cudair_linear_backward", dbias=AT + (place << 20) - 4)
+
+
+def test_matrices_side_by_side_are_not_refused(launches, cudair):
+    """Columns of one array beside one another, and one after the other: accepted up to the launch."""
+    import ctypes
+
+    from cudair import _lib
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not real")
+    for call, out, other, place in PARTIAL:
+        base = AT + (place << 20)
+        for shift in (64, -64, 32 * 128, -32 * 128, 32 * 128 - 64):
+            rc = getattr(cudair.lib(), call)(ctypes.byref(_square(call, **{out: base + shift})), None)
+            assert rc != _lib.ERR_INVALID, (call, out, other, shift, cudair.last_error())
+
+
+def test_overlap_is_exact(cudair):
+    """d and z of random pitches, types and distances: refused if and only if they have a byte in common."""
+    import ctypes
+    import random
+
+    from cudair import _lib
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not real")
+
+    def spans(at, pitch, row, rows):
+        return {at + i * pitch + j for i in range(rows) for j in range(0, row, 2)}
+
+    rng, seen = random.Random(7), [0, 0]
+    for _ in range(2500):
+        M, N, f32 = rng.choice([1, 1, 2, 3, 7]), rng.choice([1, 3, 8, 20]), rng.random() < 0.5
+        ldd, ldz = (-(-N // 8) * 8 + 8 * rng.randrange(6) for _ in range(2))
+        d, z = AT + (1 << 20), AT + (1 << 20) + 16 * rng.randrange(-30, 30)
+        args = _lib.LinearArgs(a=AT, b=AT + (8 << 20), d=d, z=z, M=M, N=N, K=8, lda=8, ldb=24, ldd=ldd, ldz=ldz,
+                               flags=0x10 if f32 else 0)
+        rc = cudair.lib().cudair_linear(ctypes.byref(args), None)
+        want = bool(spans(d, ldd * (4 if f32 else 2), N * (4 if f32 else 2), M) & spans(z, ldz * 2, N * 2, M))
+        assert (rc == _lib.ERR_INVALID) == want, (M, N, f32, ldd, ldz, z - d, cudair.last_error())
+        seen[want] += 1
+    assert min(seen) > 300
