@@ -158,3 +158,84 @@ def test_weights_written_two_kernels_before(dev, cudair, mode, last):
         kernels.set_gemm_pdl(0)
         kernels.set_linear_kernel(0)
     assert kernels.wait_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("kernel", [(SPLIT, 0), (PAIRS, 0)], ids=["split", "pairs"])
+@pytest.mark.parametrize("M,N,K", [(5, 264, 136), (1300, 2312, 1096)])
+def test_captured_behind_copies_and_joins(dev, cudair, M, N, K, kernel, mode):
+    """A capture in which calls follow a memset, a copy and the join of two streams, in each launch mode:
+    replayed, the same bits as eagerly."""
+    import torch
+    from cudair import kernels
+    bf = torch.bfloat16
+    gen = plain._gen(dev, M, 51)
+    rand = lambda r, c: torch.randn(r, c, generator=gen, device=dev).to(bf)  # noqa: E731
+    x, src, w, dy, z = torch.empty(M, K, dtype=bf, device=dev), rand(M, K), rand(N, K), rand(M, N), rand(M, N)
+    y, y2, dz, dy2 = (torch.empty(M, N, dtype=bf, device=dev) for _ in range(4))
+    da, db, dbias = torch.empty_like(x), torch.empty_like(w), torch.empty(N, device=dev)
+    outs, side = (y, y2, dz, da, db, dbias), torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        x.zero_()
+        x.copy_(src)
+        kernels.linear(x, w, y, act="silu", b_trans=True)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            torch.mul(dy, 2, out=dy2)
+            kernels.linear(x, w, y2, act="gelu", b_trans=True)
+        main.wait_stream(side)
+        kernels.linear_backward(dy2, x, w, z=z, dz=dz, da=da, db=db, dbias=dbias, act="silu", b_trans=True)
+
+    kernels.set_gemm_pdl(mode)
+    try:
+        with pinned(*kernel):
+            run()
+            torch.cuda.synchronize()
+            want = [t.clone() for t in outs]
+            for t in outs:
+                t.fill_(3.0)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                run()
+            for _ in range(3):
+                graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(t, v) for t, v in zip(outs, want))
+    finally:
+        kernels.set_gemm_pdl(0)
+    assert kernels.wait_status(clear=True) == 0
+
+
+def test_calls_from_several_threads(dev, cudair):
+    """Four host threads, a stream each."""
+    import threading
+
+    import torch
+    from cudair import kernels
+    bf = torch.bfloat16
+    x, w = torch.randn(200, 264, device=dev).to(bf), torch.randn(520, 264, device=dev).to(bf)
+    want, outs, failed = torch.empty(200, 520, dtype=bf, device=dev), [], []
+    kernels.linear(x, w, want, act="silu", b_trans=True)
+    outs = [torch.empty_like(want) for _ in range(4)]
+    torch.cuda.synchronize()
+
+    def work(o):
+        try:
+            stream = torch.cuda.Stream()
+            for _ in range(100):
+                kernels.linear(x, w, o, act="silu", b_trans=True, stream=stream)
+            stream.synchronize()
+        except Exception as e:  # a thread's own failure is not raised by join
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert all(torch.equal(o, want) for o in outs)
+    assert kernels.wait_status(clear=True) == 0
