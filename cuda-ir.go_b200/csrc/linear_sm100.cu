@@ -35,8 +35,11 @@
 //
 // Below that bound, what limits a k-block is the way from L2: 32 KB into an SM
 // in 0.29 us with few SMs busy (59 bytes a clock), 0.37 us with all (13 TB/s
-// in all).  So outputs of few tiles stay short of a kernel that shares copies
-// between CTAs (512 x 4096 x 4096: 26 us).
+// in all).  Outputs of few tiles with a long contraction are short of SMs: a tile's
+// contraction is not cut here (512 x 4096 x 4096: 44 tiles, 60 SMs idle, 26 us).
+// With a short contraction the epilogue is the longer part (8192 x 14336 x 512:
+// eight k-blocks are 3 us of a tile's 4.2 without an activation): a warp loads,
+// computes and stores one chunk after another.
 //
 // The epilogue writes each thread's row straight from registers, 32 bytes a
 // store (a whole sector): no staging in shared memory, which goes to the ring

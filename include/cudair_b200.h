@@ -400,14 +400,16 @@ int cudair_linear(const cudair_linear_args *args, void *stream);
  *   dB = A^T . dZ            (stored as B is; of A's type, or fp32 with _DB_F32)
  *   dbias[n] = sum_m dZ      (N fp32 values, from dZ before it is rounded)
  * dY is of A's type, or fp32 with CUDAIR_LINEAR_D_F32.  dz is rounded to 16
- * bits, since it is an operand of the products: it is needed where act is not
+ * bits, since it is an operand of the products (in fp16 a value beyond 65504
+ * becomes infinite and one below 2^-25 zero, even where the gradients would
+ * not): it is needed where act is not
  * CUDAIR_ACT_NONE or dY is fp32, and must be NULL otherwise (dY serves); it
  * may be dY's or z's own memory (same pitch).  z is needed where act is not
  * CUDAIR_ACT_NONE.  da, db and dbias may be NULL, and what only they need (b,
  * a) too.  Outputs are written, not added to, and their sums do not depend on
  * timing.  M of 0 gives dB = 0 and dbias = 0, N of 0 gives dA = 0; the lengths
  * that are summed over (N for dA, M for dB) are at most 2^26.  Layout rules as
- * cudair_linear.  Runs two or three kernels, the later ones launched while
+ * cudair_linear.  Runs one to three kernels, the later ones launched while
  * the ones before end, in every mode of cudair_set_gemm_pdl.
  */
 typedef struct cudair_linear_backward_args {
@@ -442,8 +444,8 @@ int cudair_gated(const cudair_gated_args *args, void *stream);
  *   dG = dH * U * act'(G),  dU = dH * act(G)   (dg, du: M x N, 16 bits)
  *   dX  = dG . Wg^T + dU . Wu^T                (M x K; fp32 with _DA_F32)
  *   dWg = X^T . dG,  dWu = X^T . dU            (as the weights; fp32 with _DB_F32)
- * dg and du are needed, and may be g's and u's (or dH's) own memory (same
- * pitch).  dx may be NULL; dwg and dwu are both given or both NULL.  N is at most
+ * dg and du are needed (rounded to 16 bits as dz is), and may be g's and u's (or
+ * dH's) own memory (same pitch).  dx may be NULL; dwg and dwu are both given or both NULL.  N is at most
  * 2^25 for dX, whose sums run over two contractions.  Other
  * rules as cudair_linear_backward.
  */
