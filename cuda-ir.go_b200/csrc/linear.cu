@@ -310,8 +310,11 @@ int check_depth(const char *op, int64_t depth, int parts = 1) {
     return CUDAIR_OK;
 }
 
+// The largest pitch, in elements: row * pitch stays far inside 64 bits.
+constexpr int64_t kMaxPitch = INT64_MAX >> 34;
+
 // Where a matrix lies, in bytes; no rows: nowhere.  (An operand that is given but not needed may
-// have no pitch: its first row counts.)
+// have no such pitch: its first row counts.)
 struct Extent {
     int64_t at = 0, pitch = 0, row = 0, rows = 0;
 };
@@ -319,9 +322,9 @@ Extent extent(const void *p, int64_t ld, int64_t rows, int64_t cols, int elem) {
     Extent e;
     if (!p || rows == 0 || cols == 0) return e;
     e.at = static_cast<int64_t>(reinterpret_cast<uintptr_t>(p));
-    e.pitch = ld * elem;
     e.row = cols * elem;
-    e.rows = ld < cols ? 1 : rows;
+    e.rows = ld < cols || ld > kMaxPitch ? 1 : rows;
+    e.pitch = e.rows > 1 ? ld * elem : e.row;
     return e;
 }
 
@@ -338,8 +341,7 @@ bool overlap(const Extent &a, const Extent &b) {
     if (a.rows == 0 || b.rows == 0) return false;
     if (a.at + (a.rows - 1) * a.pitch + a.row <= b.at || b.at + (b.rows - 1) * b.pitch + b.row <= a.at) return false;
     if (a.rows == 1 || b.rows == 1 || a.pitch == b.pitch) {
-        const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
-        return rows_meet(a, b, pitch > 0 ? pitch : 1);
+        return rows_meet(a, b, a.rows > 1 ? a.pitch : b.pitch);
     }
     const Extent &few = a.rows < b.rows ? a : b, &many = a.rows < b.rows ? b : a;
     for (int64_t i = 0; i < few.rows; ++i) {
@@ -386,7 +388,7 @@ int check_mat(const char *op, const char *name, const void *p, int64_t ld, int64
     if (ld % (16 / elem))
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: pitch %lld of %s must be a multiple of %d (16-byte rows)",
                          op, (long long)ld, name, 16 / elem);
-    if (ld > (INT64_MAX >> 34))  // row * pitch stays far inside 64 bits
+    if (ld > kMaxPitch)
         return set_error(CUDAIR_ERR_INVALID, "cudair: %s: pitch %lld of %s is too large", op, (long long)ld, name);
     return CUDAIR_OK;
 }

@@ -200,3 +200,18 @@ def test_overlap_is_exact(cudair):
         assert (rc == _lib.ERR_INVALID) == want, (M, N, f32, ldd, ldz, z - d, cudair.last_error())
         seen[want] += 1
     assert min(seen) > 300
+
+
+def test_pitches_of_operands_that_are_not_needed(cudair):
+    """Without db nothing reads a: its pitch is not looked at, and only its first row is kept clear of."""
+    import ctypes
+
+    from cudair import _lib
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are not real")
+    for ld in (0, -8, 7, 2 ** 29 + 8, 2 ** 61 + 3, 2 ** 63 - 1):
+        args = _square("cudair_linear_backward", db=None, lda=ld)
+        assert cudair.lib().cudair_linear_backward(ctypes.byref(args), None) != _lib.ERR_INVALID, (ld, cudair.last_error())
+        assert "da lies over another" in _refused(cudair, "cudair_linear_backward", db=None, lda=ld,
+                                                  da=AT + (1 << 20) + 48)
